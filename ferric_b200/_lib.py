@@ -32,6 +32,18 @@ class ChainLink(C.Structure):
                 ("h_dev", C.c_void_p), ("norm_weight_dev", C.c_void_p)]
 
 
+class KvCache(C.Structure):
+    """``ferric_kv_cache`` of include/ferric_cuda.h."""
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("ggml_type", C.c_uint32), ("n_pages", C.c_size_t),
+                ("page_size", C.c_size_t), ("n_heads", C.c_size_t), ("head_dim", C.c_size_t), ("page_stride", C.c_size_t)]
+
+
+class KvSeqs(C.Structure):
+    """``ferric_kv_seqs`` of include/ferric_cuda.h."""
+    _fields_ = [("page_table_dev", C.c_void_p), ("n_seqs", C.c_size_t), ("max_pages", C.c_size_t), ("table_stride", C.c_size_t),
+                ("lens_dev", C.c_void_p), ("starts_dev", C.c_void_p)]
+
+
 class GgufTensor(C.Structure):
     _fields_ = [("name", C.c_char_p), ("n_dims", C.c_uint32), ("dims", C.c_uint64 * 4), ("ggml_type", C.c_uint32),
                 ("offset", C.c_uint64), ("n_elements", C.c_uint64), ("nbytes", C.c_uint64)]
@@ -80,6 +92,11 @@ SIGNATURES = {
     "ferric_cuda_swiglu": (_I32, [_P, _P, _SZ, _SZ, _P]),
     "ferric_cuda_matmul_q_swiglu_id": (_I32, [_P, _P, _P, _SZ, _SZ, _P, _SZ, _SZ, _P]),
     "ferric_cuda_matmul_q_id_wsum": (_I32, [_P, _P, _P, _SZ, _SZ, _SZ, _P, _SZ, _P]),
+    "ferric_cuda_rope_create": (_I32, [_P, _SZ, C.c_double, _P, _I32, C.POINTER(_P)]),
+    "ferric_cuda_rope_free": (None, [_P]),
+    "ferric_cuda_kv_append": (_I32, [_P, C.POINTER(KvCache), C.POINTER(KvSeqs), _P, _P, _SZ, _P, _SZ, _SZ]),
+    "ferric_cuda_kv_attend": (_I32, [_P, C.POINTER(KvCache), C.POINTER(KvSeqs), _P, _P, _SZ, _SZ, _SZ, C.c_float, _SZ, _P, _U32, _SZ]),
+    "ferric_cuda_attend_reserve": (_I32, [_P]),
     "ferric_cuda_tp_create": (_I32, [_P, _I32, _I32, _SZ, C.POINTER(_P)]),
     "ferric_cuda_tp_export": (_I32, [_P, _P]),
     "ferric_cuda_tp_connect": (_I32, [_P, _P]),

@@ -408,6 +408,7 @@ void ferric_cuda_ctx_free(ferric_cuda_ctx* ctx)
     cudaStreamSynchronize(ctx->stream);
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->tune.split_ws.partial) cudaFree(ctx->tune.split_ws.partial);
+    if (ctx->attend_ws) cudaFree(ctx->attend_ws);
     if (ctx->owns_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
 }

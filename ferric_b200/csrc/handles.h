@@ -28,6 +28,7 @@ struct ferric_cuda_ctx {
     float* chain_ssq = nullptr;
     unsigned* chain_tickets = nullptr;
     unsigned* chain_done = nullptr;
+    void* attend_ws = nullptr;   // pieces of rows that several CTAs attend to, and their tickets (ferric_cuda_attend_reserve)
 };
 
 struct ferric_qmatrix {
@@ -36,6 +37,13 @@ struct ferric_qmatrix {
     ferric::DeviceWeights w;
     void* storage = nullptr;
     size_t storage_bytes = 0;
+};
+
+// The rotation's frequencies on one device (ferric_cuda_rope_*).
+struct ferric_rope {
+    int device = 0;
+    int rotary = 0, interleaved = 0;
+    double* turns = nullptr;   // [rotary / 2] turns per position
 };
 
 // Proj (crates/ferric-llama/src/qwen3.rs:192-228): one logical projection whose stacked outputs live in one matrix

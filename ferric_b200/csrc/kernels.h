@@ -4,6 +4,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "kv_index.h"
+
 namespace ferric {
 
 constexpr uint32_t kGgmlF32 = 0, kGgmlQ8_0 = 8, kGgmlQ4K = 12, kGgmlQ5K = 13, kGgmlQ6K = 14;
@@ -204,6 +206,22 @@ size_t gemv_tc_scratch_bytes(uint32_t ty, const DeviceWeights& w, size_t m, Epil
 int32_t launch_gemv_tc(cudaStream_t st, uint32_t ty, const DeviceWeights& w, const float* x, size_t m, size_t ldx, float* y, size_t ldy,
                        Epilogue epi, void* scratch, const GemvTuning& tune, int* launches, const WideDst* scatter = nullptr,
                        bool* scattered = nullptr);
+// ---- the paged key-value cache and the attention over it (kernels_kv.cu, kernels_attend.cu) -----------------------
+int32_t launch_kv_append(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const float* k, size_t ldk,
+                         const float* v, size_t ldv, const GemvTuning& tune);
+struct AttendArgs {
+    const float* q = nullptr;
+    size_t ldq = 0;
+    void* out = nullptr;
+    size_t ldo = 0;
+    bool out_bf16 = false;
+    int heads = 0;                   // query heads, a multiple of the cache's
+    float scale = 0.0f;
+    int window = 0;                  // keys a token sees at most; 0: all up to its own
+};
+int32_t launch_attend(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a,
+                      const GemvTuning& tune, int* launches);
+
 // Synchronise the stream and fetch-and-clear the code a GEMM CTA left when one of its bounded waits ran out.
 int32_t gemm_status(cudaStream_t st, int* code);
 

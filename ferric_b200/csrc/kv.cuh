@@ -1,0 +1,94 @@
+// What the kernels over the paged key-value cache share: the views they are given, the position rotation and the plain
+// evaluation of one query row.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace ferric {
+
+// cos and sin of pos * frequency.  The frequencies are held in turns per position in 64 bits: a float product is off by
+// 2^-24 of the whole angle, which at position 10^5 is 6e-3 rad; here the whole turns are dropped in 64 bits and the
+// rest, at most half a turn, is rounded to a float once.
+__device__ __forceinline__ void rope_cos_sin(double turns_per_pos, int pos, float* c, float* s)
+{
+    const double t = (double)pos * turns_per_pos;
+    sincospif(2.0f * (float)(t - rint(t)), s, c);
+}
+// Rotation partner of element e of a head and where their pair sits among the frequencies; e >= rotary: not rotated.
+__device__ __forceinline__ float rope_element(const RopeView& r, const float* x, int e, int pos)
+{
+    if (e >= r.rotary) return x[e];
+    float c, s;
+    if (r.interleaved) {
+        rope_cos_sin(r.turns[e >> 1], pos, &c, &s);
+        return (e & 1) ? fmaf(x[e - 1], s, x[e] * c) : fmaf(-x[e + 1], s, x[e] * c);
+    }
+    const int half = r.rotary >> 1;
+    rope_cos_sin(r.turns[e < half ? e : e - half], pos, &c, &s);
+    return e < half ? fmaf(-x[e + half], s, x[e] * c) : fmaf(x[e - half], s, x[e] * c);
+}
+
+__device__ __forceinline__ float kv_to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float kv_to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void kv_from_float(float v, __half* o) { *o = __float2half_rn(v); }
+__device__ __forceinline__ void kv_from_float(float v, __nv_bfloat16* o) { *o = __float2bfloat16_rn(v); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// One query row against keys [lo, hi) of one sequence and head, by one warp, in f32: the definition, key by key.  `q` is
+// the rotated row times scale * log2(e), in shared memory.  Lane = key for the scores, lane = dimension for the sums, so a
+// masked or absent key is never multiplied by anything.  Leaves the running maximum (log2 units), the sum and the
+// unnormalised output (element lane + 32 e).
+template <typename T, int D>
+__device__ __forceinline__ void attend_row_plain(const KvCacheView& c, const KvSeqsView& s, int seq, int h, const float* q, int lo, int hi,
+                                                 int lane, float* m_out, float* l_out, float (&acc)[D / 32])
+{
+    const T* K = reinterpret_cast<const T*>(c.k);
+    const T* V = reinterpret_cast<const T*>(c.v);
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) acc[e] = 0.0f;
+    for (int k0 = lo; k0 < hi; k0 += 32) {
+        const int key = k0 + lane;
+        const long long off = key < hi ? kv_offset(c, s, seq, h, key) : -1;
+        float dot = -INFINITY;
+        if (off >= 0) {
+            dot = 0.0f;
+            for (int d = 0; d < D; d += 8) {
+                const uint4 w = *reinterpret_cast<const uint4*>(K + off + d);
+                const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                for (int i = 0; i < 8; i++) dot = fmaf(q[d + i], kv_to_float(e[i]), dot);
+            }
+        }
+        float mx = dot;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        mx = fmaxf(mx, m);
+        const float base = mx == -INFINITY ? 0.0f : mx;   // nothing seen yet: every term below is 0
+        const float fix = exp2f(m - base);
+        const float p = off >= 0 ? exp2f(dot - base) : 0.0f;
+        l = l * fix + p;
+        m = mx;
+#pragma unroll
+        for (int e = 0; e < D / 32; e++) acc[e] *= fix;
+        const unsigned have = __ballot_sync(0xffffffffu, off >= 0);
+        for (int i = 0; i < 32; i++) {
+            if (!((have >> i) & 1u)) continue;
+            const float pi = __shfl_sync(0xffffffffu, p, i);
+            const long long oi = __shfl_sync(0xffffffffu, off, i);
+#pragma unroll
+            for (int e = 0; e < D / 32; e++) acc[e] = fmaf(pi, kv_to_float(V[oi + lane + 32 * e]), acc[e]);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    *m_out = m;
+    *l_out = l;
+}
+
+}  // namespace ferric

@@ -1,0 +1,100 @@
+// Index arithmetic of the paged key-value cache and of the attention's work split: plain integer code shared by the device
+// kernels, the host launchers and a CPU test.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#if defined(__CUDACC__)
+#define FERRIC_KV_HD __host__ __device__ __forceinline__
+#else
+#define FERRIC_KV_HD inline
+#endif
+
+namespace ferric {
+
+// Keys and values of one layer: [n_pages][heads][page][dim] each, pages `page_stride` elements apart.
+struct KvCacheView {
+    void* k = nullptr;
+    void* v = nullptr;
+    long long page_stride = 0;
+    int n_pages = 0, page_shift = 0, heads = 0, dim = 0;
+    int bf16 = 0;                    // 1: bf16, 0: f16
+};
+// The batch: table[seq][cols] page numbers, lengths (new tokens included), first token row of each sequence (null: token
+// row i is the one new token of sequence i); `tokens` rows of activations in all.
+struct KvSeqsView {
+    const int* table = nullptr;
+    long long table_stride = 0;
+    const int* lens = nullptr;
+    const int* starts = nullptr;
+    int cols = 0, seqs = 0, tokens = 0;
+};
+struct RopeView {
+    const double* turns = nullptr;   // [rotary / 2] turns per position
+    int rotary = 0;                  // leading elements of a head that are rotated; 0: none
+    int interleaved = 0;             // 1: pairs (2i, 2i + 1), 0: pairs (i, i + rotary / 2)
+};
+
+FERRIC_KV_HD int kv_min(int a, int b) { return a < b ? a : b; }
+FERRIC_KV_HD int kv_max(int a, int b) { return a > b ? a : b; }
+
+// The new tokens of sequence i: activation rows [first, first + n), the last of them at position len - 1.
+struct KvSpan {
+    int first, n, len;
+    // position of new token j; a length shorter than the new tokens puts the first of them below 0, where nothing is
+    FERRIC_KV_HD int pos(int j) const { return (int)((long long)len - n + j < INT32_MIN ? INT32_MIN : (long long)len - n + j); }
+};
+FERRIC_KV_HD KvSpan kv_span(const KvSeqsView& s, int i)
+{
+    KvSpan r;
+    if (s.starts) {
+        // starts that do not ascend, or reach past the activations, yield empty spans, never a row outside them
+        const int a = kv_max(0, s.starts[i]), b = kv_min(s.tokens, s.starts[i + 1]);
+        r.first = a;
+        r.n = b > a ? b - a : 0;
+    } else {
+        r.first = i;
+        r.n = 1;
+    }
+    r.len = s.lens[i];
+    return r;
+}
+// The sequence whose span holds activation row t, or -1 (rows before the first start and behind the last one).
+FERRIC_KV_HD int kv_seq_of(const KvSeqsView& s, int t)
+{
+    if (!s.starts) return t < s.seqs ? t : -1;
+    if (t < s.starts[0] || t >= s.starts[s.seqs]) return -1;
+    int lo = 0, hi = s.seqs;   // starts[lo] <= t < starts[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s.starts[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+// The cache page of column `col` of sequence `seq`, or -1 where the table has none.
+FERRIC_KV_HD int kv_page(const KvCacheView& c, const KvSeqsView& s, int seq, int col)
+{
+    if (col < 0 || col >= s.cols) return -1;
+    const int page = s.table[(long long)seq * s.table_stride + col];
+    return (unsigned)page < (unsigned)c.n_pages ? page : -1;
+}
+// First element of (page of position `pos`, head h, slot of `pos`), or -1 where there is no page.  64-bit: a cache passes
+// 2^31 elements at 4 GB.
+FERRIC_KV_HD long long kv_offset(const KvCacheView& c, const KvSeqsView& s, int seq, int h, int pos)
+{
+    const int page = pos < 0 ? -1 : kv_page(c, s, seq, pos >> c.page_shift);
+    if (page < 0) return -1;
+    return (long long)page * c.page_stride + (((long long)h << c.page_shift) + (pos & ((1 << c.page_shift) - 1))) * c.dim;
+}
+// Keys a token at position `pos` sees: [lo, hi).  The table's capacity (at most kKvMaxPositions) bounds hi; a window of w keys
+// bounds lo.
+constexpr long long kKvMaxPositions = 1ll << 30;
+FERRIC_KV_HD int kv_seen_lo(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
+FERRIC_KV_HD int kv_seen_hi(const KvCacheView& c, const KvSeqsView& s, int pos)
+{
+    const long long cap = (long long)s.cols << c.page_shift, h = pos < 0 ? 0 : (long long)pos + 1;
+    return (int)(h < cap ? h : cap);
+}
+
+}  // namespace ferric

@@ -1,6 +1,7 @@
 """Python mirror of the reference's QMatrix / matmul_q operator interface (see package docstring)."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from typing import Optional
@@ -458,6 +459,164 @@ class Proj:
             self.close()
         except Exception:
             pass
+
+
+class Rope:
+    """The position rotation of queries and keys (``ferric_cuda_rope_*``): the first ``rotary`` elements of a head turn by
+    position * frequency, in pairs (i, i + rotary / 2), or (2i, 2i + 1) when ``interleaved``.  Frequencies are
+    ``base ** (-2i / rotary)`` radians per position, or ``inv_freq`` (rotary / 2 numbers) where given."""
+
+    def __init__(self, ctx: Context, rotary: int, base: float = 10000.0, interleaved: bool = False, inv_freq=None):
+        self._lib = ctx._lib
+        self.device, self.rotary, self.interleaved = ctx.device, int(rotary), bool(interleaved)
+        f = None
+        if inv_freq is not None:
+            f = np.ascontiguousarray(inv_freq.detach().cpu().numpy() if isinstance(inv_freq, torch.Tensor) else inv_freq, dtype=np.float64)
+            if f.shape != (self.rotary // 2,):
+                raise ValueError(f"inv_freq holds {f.shape} numbers, rotary = {rotary} takes {self.rotary // 2}")
+        h = C.c_void_p()
+        _check(self._lib.ferric_cuda_rope_create(ctx._h, self.rotary, float(base), f.ctypes.data if f is not None else None,
+                                                 int(interleaved), C.byref(h)), "Rope")
+        self._h = h
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            self._lib.ferric_cuda_rope_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KVSeqs:
+    """The batch a cache call works on (``ferric_kv_seqs``), int32 CUDA tensors read when the kernels run: ``page_table``
+    [n_seqs, max_pages]; ``lens`` [n_seqs], each sequence's length with its new tokens; ``starts`` [n_seqs + 1], the first
+    activation row of each sequence, or None when row i is the one new token of sequence i."""
+
+    def __init__(self, page_table: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None):
+        for name, t, dim in (("page_table", page_table, 2), ("lens", lens, 1), ("starts", starts, 1)):
+            if t is None and name == "starts":
+                continue
+            if not (t.is_cuda and t.dtype == torch.int32 and t.dim() == dim and (t.stride(-1) == 1 or t.shape[-1] <= 1)):
+                raise TypeError(f"{name} must be a {dim}-D int32 CUDA tensor with adjacent elements")
+        if lens.shape[0] != page_table.shape[0] or (starts is not None and starts.shape[0] != lens.shape[0] + 1):
+            raise ValueError("page_table, lens and starts disagree about the number of sequences")
+        if lens.device != page_table.device or (starts is not None and starts.device != lens.device):
+            raise ValueError("page_table, lens and starts must be on one device")
+        self.page_table, self.lens, self.starts = page_table, lens, starts
+        n, cols = page_table.shape
+        self._c = _lib.KvSeqs(page_table.data_ptr(), n, cols, page_table.stride(0) if n > 1 else 0, lens.data_ptr(),
+                              starts.data_ptr() if starts is not None else None)
+
+
+class KVCache:
+    """One layer's paged key-value cache (``ferric_kv_cache``): ``k`` and ``v`` [n_pages, n_kv_heads, page_size, head_dim] in
+    float16 or bfloat16, the caller's tensors (pages may lie apart: views of one allocation for all layers are fine).
+
+    ``append`` and ``attend`` run on the context's stream, ordered with torch's current one where that is another; both take
+    column slices of a fused q|k|v result in place."""
+
+    def __init__(self, ctx: Context, k: torch.Tensor, v: torch.Tensor):
+        if k.dtype not in (torch.float16, torch.bfloat16) or v.dtype != k.dtype or k.dim() != 4 or v.shape != k.shape:
+            raise TypeError("k and v must be float16 or bfloat16 tensors [n_pages, n_kv_heads, page_size, head_dim] of one type and shape")
+        n_pages, heads, page, dim = k.shape
+        for t in (k, v):
+            if not t.is_cuda or t.device.index != ctx.device:
+                raise ValueError(f"the cache is on {t.device}, the context on device {ctx.device}")
+            if any(n > 1 and st != want for n, st, want in zip(t.shape[1:], t.stride()[1:], (page * dim, dim, 1))):
+                raise ValueError("the heads of a page must lie densely, as [n_kv_heads, page_size, head_dim]")
+        if n_pages > 1 and k.stride(0) != v.stride(0):
+            raise ValueError("k and v must have one page stride")
+        self.ctx, self._lib, self.k, self.v = ctx, ctx._lib, k, v
+        self.n_heads, self.page_size, self.head_dim = heads, page, dim
+        self._c = _lib.KvCache(k.data_ptr(), v.data_ptr(), GGML_F16 if k.dtype == torch.float16 else GGML_BF16, n_pages, page, heads,
+                               dim, k.stride(0) if n_pages > 1 else 0)
+
+    @classmethod
+    def empty(cls, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+              dtype: torch.dtype = torch.bfloat16) -> "KVCache":
+        """A cache over memory of its own; nothing of it is read before it has been appended."""
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        dev = torch.device("cuda", ctx.device)
+        return cls(ctx, torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
+
+    def _rows(self, x: torch.Tensor, name: str) -> torch.Tensor:
+        if not x.is_cuda or x.dtype != torch.float32 or x.dim() not in (2, 3):
+            raise TypeError(f"{name} must be a float32 CUDA tensor [tokens, heads * head_dim] or [tokens, heads, head_dim]")
+        if x.dim() == 3:
+            if x.shape[2] != self.head_dim:
+                raise ValueError(f"{name} has heads of {x.shape[2]}, the cache of {self.head_dim}")
+            x = x.flatten(1) if x.stride(2) == 1 and (x.shape[1] <= 1 or x.stride(1) == self.head_dim) else x.contiguous().flatten(1)
+        if x.device.index != self.ctx.device:
+            raise ValueError(f"{name} is on {x.device}, the context on device {self.ctx.device}")
+        ok = (x.shape[1] <= 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % 4 == 0)) \
+            and x.data_ptr() % 16 == 0
+        return x if ok else x.contiguous()
+
+    @contextlib.contextmanager
+    def _ordered(self):
+        """Where the context's stream is not torch's current one: the call waits for what torch has queued there, and what torch
+        queues next waits for the call, so operands and results may be made and dropped as if it ran on that stream."""
+        st = self._lib.ferric_cuda_ctx_stream(self.ctx._h) or 0
+        cur = torch.cuda.current_stream(self.ctx.device)
+        if st == cur.cuda_stream:
+            yield
+            return
+        own = torch.cuda.ExternalStream(st, device=self.ctx.device) if st else torch.cuda.default_stream(self.ctx.device)
+        own.wait_stream(cur)
+        try:
+            yield
+        finally:
+            cur.wait_stream(own)
+
+    def _common(self, seqs: KVSeqs, rope: Optional[Rope]):
+        if seqs.lens.device.index != self.ctx.device:
+            raise ValueError(f"the sequences are on {seqs.lens.device}, the context on device {self.ctx.device}")
+        return C.byref(self._c), C.byref(seqs._c), rope._h if rope is not None else None
+
+    def append(self, seqs: KVSeqs, k: torch.Tensor, v: torch.Tensor, rope: Optional[Rope] = None) -> None:
+        """Store the new tokens' keys (rotated by ``rope``) and values at their positions (``ferric_cuda_kv_append``)."""
+        k, v = self._rows(k, "k"), self._rows(v, "v")
+        cols = self.n_heads * self.head_dim
+        if k.shape[1] != cols or v.shape != k.shape:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {cols}]")
+        c, s, r = self._common(seqs, rope)
+        n = k.shape[0]
+        with self._ordered():
+            _check(self._lib.ferric_cuda_kv_append(self.ctx._h, c, s, r, k.data_ptr(), k.stride(0) if n > 1 else 0, v.data_ptr(),
+                                                   v.stride(0) if n > 1 else 0, n), "kv_append")
+
+    def attend(self, seqs: KVSeqs, q: torch.Tensor, rope: Optional[Rope] = None, scale: Optional[float] = None, window: int = 0,
+               out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Attention of the new tokens over what the cache holds (``ferric_cuda_kv_attend``): q [tokens, heads * head_dim],
+        rotated by ``rope``; each token sees its sequence's keys up to its own position, the last ``window`` of them where
+        that is set.  Returns [tokens, heads * head_dim] in ``out_dtype`` (float32, or bfloat16 for the prefill products),
+        or fills ``out``; rows of no sequence are left as they were (in a result made here: as the memory was)."""
+        q = self._rows(q, "q")
+        n, cols = q.shape
+        if cols % self.head_dim != 0:
+            raise ValueError(f"q has {cols} columns, heads have {self.head_dim}")
+        if window < 0:
+            raise ValueError("window must not be negative")
+        if out is None:
+            out = torch.empty((n, cols), dtype=out_dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16) or out.device != q.device or \
+                (out.stride(1) != 1 and cols > 1):
+            raise TypeError("out must be a float32 or bfloat16 tensor of q's shape and device with adjacent columns")
+        if out.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("out_dtype must be float32 or bfloat16")
+        if scale is not None and scale == 0.0:
+            raise ValueError("scale must not be 0 (None = 1 / sqrt(head_dim))")
+        c, s, r = self._common(seqs, rope)
+        with self._ordered():
+            _check(self._lib.ferric_cuda_kv_attend(self.ctx._h, c, s, r, q.data_ptr(), q.stride(0) if n > 1 else 0, n, cols // self.head_dim,
+                                                   float(scale) if scale is not None else 0.0, int(window), out.data_ptr(),
+                                                   GGML_F32 if out.dtype == torch.float32 else GGML_BF16,
+                                                   out.stride(0) if n > 1 else 0), "kv_attend")
+        return out
 
 
 class _DevView:

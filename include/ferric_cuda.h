@@ -325,6 +325,66 @@ int32_t ferric_cuda_dequant_f32(ferric_cuda_ctx *ctx, const ferric_qmatrix *qm, 
  * (crates/ferric-tensor/src/dtype.rs:4159-4163): out[rows * cols] uint16 bf16 bits. */
 int32_t ferric_cuda_dequant_bf16(ferric_cuda_ctx *ctx, const ferric_qmatrix *qm, uint16_t *out_dev);
 
+/* ---- the paged key-value cache and attention over it ---------------------------------------- */
+/* The mixer between a layer's q|k|v and o products (Qwen35::attn, crates/ferric-llama/src/qwen35.rs:665-724; split-KV
+ * decode attention, crates/ferric-tensor/src/lib.rs:743-788): the new tokens' keys and values are appended to the layer's
+ * cache, rotated on the way, and the new tokens attend to what the cache holds.  The same two calls serve a decode step
+ * (one new token per sequence), the check of drafted tokens (a few) and a prompt or a chunk of one (many).
+ *
+ * Rotation (RoPE): the first `rotary` elements of a head are turned by position * frequency, in pairs (i, i + rotary / 2),
+ * or (2i, 2i + 1) when interleaved.  Pair i's frequency is base^(-2i / rotary) radians per position, or inv_freq[i] (HOST,
+ * rotary / 2 doubles, copied) where that is given: scaled variants pass their own.  Angles are taken in 64 bits, so far
+ * positions lose nothing.  rotary: a multiple of 16.  A ferric_rope is immutable and may be used by any context on its
+ * device; creating one allocates and synchronises (not during capture). */
+typedef struct ferric_rope ferric_rope;
+int32_t ferric_cuda_rope_create(ferric_cuda_ctx *ctx, size_t rotary, double base, const double *inv_freq, int32_t interleaved,
+                                ferric_rope **out);
+void ferric_cuda_rope_free(ferric_rope *r);
+
+/* One layer's cache, in memory of the caller's: k and v [n_pages][n_heads][page_size][head_dim] each, in f16 or bf16, 16-byte
+ * aligned, `page_stride` elements (a multiple of 8; 0 = dense) from page to page.  page_size 16, 32, 64, 128 or 256; head_dim
+ * 64, 128 or 256; n_heads = the model's key-value heads. */
+typedef struct ferric_kv_cache {
+    void *k_dev, *v_dev;
+    uint32_t ggml_type;           /* FERRIC_GGML_F16 or FERRIC_GGML_BF16 */
+    size_t n_pages, page_size, n_heads, head_dim, page_stride;
+} ferric_kv_cache;
+/* The batch, all on the device and read when the kernels run, so a captured call follows what the host or an earlier
+ * kernel writes there: page_table[n_seqs][max_pages] (int32, rows `table_stride` apart, 0 = dense) holds the page of
+ * positions [c * page_size, (c + 1) * page_size) in column c; lens[n_seqs] each sequence's length, its new tokens included;
+ * starts[n_seqs + 1] the first activation row of each sequence (ascending), or NULL when activation row i is the one new
+ * token of sequence i (then n_tokens must equal n_seqs).  Token j of the n new tokens of a sequence of length L is at
+ * position L - n + j.  Any page number is safe: one outside [0, n_pages) -- a page given back, an unused column -- marks its
+ * positions as absent: nothing is appended there and no token sees them; the same holds for positions past max_pages
+ * and below 0.  Several sequences may share pages for reading; two tokens appended to one slot race.  max_pages * page_size at most 2^30. */
+typedef struct ferric_kv_seqs {
+    const int32_t *page_table_dev;
+    size_t n_seqs, max_pages, table_stride;
+    const int32_t *lens_dev;
+    const int32_t *starts_dev;
+} ferric_kv_seqs;
+
+/* Append: k[n_tokens, n_heads * head_dim] (rotated by `rope`; NULL = as it is) and v, both f32 with row strides ldk / ldv
+ * (multiples of 4; 0 = dense) and 16-byte aligned -- column slices of a fused q|k|v result -- are rounded to the cache's type
+ * (nearest even) and stored at their tokens' positions.  Rows outside every sequence are ignored. */
+int32_t ferric_cuda_kv_append(ferric_cuda_ctx *ctx, const ferric_kv_cache *cache, const ferric_kv_seqs *seqs, const ferric_rope *rope,
+                              const float *k_dev, size_t ldk, const float *v_dev, size_t ldv, size_t n_tokens);
+
+/* Attend: out[t, n_q_heads * head_dim] = softmax(scale * R(pos_t) q_t . K) V over the keys token t sees -- those of its
+ * sequence at positions <= its own, the last `window` of them where window > 0 -- query head h reading key-value head
+ * h / (n_q_heads / cache heads).  q is f32 like k above (rotated here: `rope` as for append); scale 0 = 1 / sqrt(head_dim).
+ * out is FERRIC_GGML_F32 (the decode products' activation type: the whole product is then kept to f32 accuracy) or
+ * FERRIC_GGML_BF16 (the prefill products'), 16-byte aligned with row stride ldo (0 = dense; a multiple of 16 bytes), and
+ * must not overlap q.  A token that sees no key gets zeros; output rows outside every sequence are left as they were.  The
+ * new tokens' own keys must have been appended.  A key or value element that is not finite reaches only the tokens that see it.
+ * Calls on one context share a workspace (ferric_cuda_attend_reserve, allocated by the first call otherwise, which must then
+ * not be under capture): graphs captured on one context must not be replayed at the same time -- give each stream of
+ * replays a context of its own.  Waits inside the kernels are bounded; ferric_cuda_gemm_status reports one that ran out. */
+int32_t ferric_cuda_kv_attend(ferric_cuda_ctx *ctx, const ferric_kv_cache *cache, const ferric_kv_seqs *seqs, const ferric_rope *rope,
+                              const float *q_dev, size_t ldq, size_t n_tokens, size_t n_q_heads, float scale, size_t window,
+                              void *out_dev, uint32_t out_type, size_t ldo);
+int32_t ferric_cuda_attend_reserve(ferric_cuda_ctx *ctx);
+
 /* ---- GGUF ingest --------------------------------------------------------------------------- */
 /* ferric_gguf::parse   crates/ferric-gguf/src/lib.rs:105-132 (bounds-safe cursor :59-103, stride guard
  * :387-431): header, metadata and tensor table of a GGUF file held in memory.  `bytes` is borrowed:

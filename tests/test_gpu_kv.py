@@ -1,0 +1,528 @@
+"""The paged key-value cache (append with rotation) and the attention over it against a 64-bit evaluation, through the
+framework's entry points, at the lengths, head layouts, pages and masks where such operators go wrong.  Tolerances are
+derived in ``kv_ref``."""
+import random
+
+import pytest
+import torch
+
+import kv_ref as R
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def F():
+    import ferric_b200
+    return ferric_b200
+
+
+@pytest.fixture()
+def ctx(F):
+    c = F.Context(0)
+    yield c
+    c.close()
+
+
+class Batch:
+    """Random inputs of one call: caches whose unused slots hold NaN, a shuffled page table, a fused q|k|v result."""
+
+    def __init__(self, F, ctx, lens, new=None, heads=8, kv_heads=2, dim=128, page=16, dtype=BF, rotary=None, interleaved=False, seed=0,
+                 pad_rows=0, spare_cols=1, base=10000.0, fill=True, interleave_pages=False):
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.heads, self.hk, self.dim, self.page, self.dtype = list(lens), heads, kv_heads, dim, page, dtype
+        self.new = [1] * len(lens) if new is None else list(new)
+        self.starts = None
+        if new is not None:
+            self.starts = [0]
+            for n in self.new:
+                self.starts.append(self.starts[-1] + n)
+        self.tokens = sum(self.new) + pad_rows
+        used = [max(0, -(-n // page)) for n in self.lens]
+        n_pages = sum(used) + 2
+        cols = max(used + [1]) + spare_cols
+        ids = random.Random(seed).sample(range(n_pages), n_pages)
+        self.table = torch.full((len(lens), cols), -1, dtype=torch.int32)
+        at = 0
+        for i, u in enumerate(used):
+            self.table[i, :u] = torch.tensor(ids[at:at + u], dtype=torch.int32)
+            at += u
+        shape = (n_pages, kv_heads, page, dim)
+        if interleave_pages:                         # k and v of a page side by side in one allocation
+            both = torch.full((n_pages, 2) + shape[1:], float("nan"), dtype=dtype, device="cuda")
+            k, v = both[:, 0], both[:, 1]
+        else:
+            k = torch.full(shape, float("nan"), dtype=dtype, device="cuda")
+            v = torch.full(shape, float("nan"), dtype=dtype, device="cuda")
+        if fill:
+            for i, n in enumerate(self.lens):
+                for c in range(used[i]):
+                    m = min(page, n - c * page)
+                    pg = int(self.table[i, c])
+                    k[pg, :, :m] = torch.randn((kv_heads, m, dim), generator=g).to(dtype).cuda()
+                    v[pg, :, :m] = torch.randn((kv_heads, m, dim), generator=g).to(dtype).cuda()
+        self.qkv = torch.randn((self.tokens, (heads + 2 * kv_heads) * dim), generator=g).cuda()
+        h, w = heads * dim, kv_heads * dim
+        self.q, self.k, self.v = self.qkv[:, :h], self.qkv[:, h:h + w], self.qkv[:, h + w:]
+        self.cache = F.KVCache(ctx, k, v)
+        dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+        self.seqs = F.KVSeqs(self.table.cuda(), dev(self.lens), None if self.starts is None else dev(self.starts))
+        rotary = dim if rotary is None else rotary
+        self.rope = F.Rope(ctx, rotary, base=base, interleaved=interleaved) if rotary else None
+        self.rope_ref = dict(rotary=rotary, base=base, interleaved=interleaved) if rotary else dict(rotary=0)
+
+    def check_attend(self, window=0, out_dtype=torch.float32, scale=None):
+        mark = torch.full((self.tokens, self.heads * self.dim), 7.0, dtype=out_dtype, device="cuda")
+        y = self.cache.attend(self.seqs, self.q, rope=self.rope, window=window, scale=scale, out=mark)
+        assert y is mark
+        want, bound, mine = R.attend(self.cache.k, self.cache.v, self.table, self.lens, self.starts, self.q, self.heads, self.rope_ref,
+                                     scale=scale, window=window, out_dtype=out_dtype)
+        got = y.double().cpu()
+        assert (got[~mine] == 7.0).all()             # rows of no sequence are left as they were
+        off = (got - want)[mine].abs()
+        assert torch.isfinite(got[mine]).all()
+        assert (off <= bound[mine]).all(), f"worst {float((off / bound[mine].clamp(min=1e-30)).max()):.3g} of the bound"
+        return y
+
+
+# ---- append -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rotary,page,kv_heads", [(128, 128, 16, 8), (64, 32, 64, 1), (256, 64, 32, 3), (128, 0, 128, 2), (64, 64, 256, 2)])
+def test_append_rotates_and_rounds_once(F, ctx, dtype, interleaved, dim, rotary, page, kv_heads):
+    b = Batch(F, ctx, lens=[1, 37, 300, 16], new=[1, 5, 290, 16], dim=dim, rotary=rotary, page=page, kv_heads=kv_heads, heads=kv_heads,
+              dtype=dtype, interleaved=interleaved, fill=False, pad_rows=3)
+    check_append(b)
+
+
+def check_append(b):
+    kx, vx, bound, written = R.append(b.cache.k, b.cache.v, b.table, b.lens, b.starts, b.k, b.v, b.rope_ref)
+    k0, v0 = b.cache.k.clone(), b.cache.v.clone()
+    b.cache.append(b.seqs, b.k, b.v, rope=b.rope)
+    u, tiny = R.U[b.dtype], 2.0 ** -25 if b.dtype == HF else 0.0
+    k, v = b.cache.k.double().cpu(), b.cache.v.double().cpu()
+    w = written
+    assert ((k - kx)[w].abs() <= bound[w] + u * (kx[w].abs() + bound[w]) + tiny).all()
+    assert ((v - vx)[w].abs() <= u * vx[w].abs() + tiny).all()
+    same = lambda a, c: torch.equal(a.view(torch.int16).cpu()[~w], c.view(torch.int16).cpu()[~w])
+    assert same(b.cache.k, k0) and same(b.cache.v, v0)        # nothing else was touched
+    return w
+
+
+def test_append_one_token_per_sequence_and_far_positions(F, ctx):
+    b = Batch(F, ctx, lens=[1, 2, 16, 17, 100001, 65536], page=256, base=1e6, fill=False)
+    assert check_append(b).sum() == 6 * b.hk * b.dim
+
+
+def test_append_skips_what_has_no_page(F, ctx):
+    b = Batch(F, ctx, lens=[40, 20, 3, 0], new=[10, 20, 8, 4], fill=False)
+    b.table[0, 2] = 10 ** 6                                    # positions 32..39 of the first sequence
+    b.table[1, 0] = -5
+    b.seqs.page_table.copy_(b.table)
+    w = check_append(b)                                        # third: positions -5..-1 do not exist; fourth: none does
+    assert w.sum() == (2 + 4 + 3) * b.hk * b.dim
+
+
+def test_append_into_pages_that_lie_apart(F, ctx):
+    check_append(Batch(F, ctx, lens=[50, 33], new=[50, 2], interleave_pages=True, fill=False, page=32))
+
+
+def test_append_takes_given_frequencies(F, ctx):
+    f = [1.0 / (3.0 + i) for i in range(32)]
+    b = Batch(F, ctx, lens=[70], new=[70], dim=64, fill=False)
+    b.rope = F.Rope(ctx, 64, inv_freq=f)
+    b.rope_ref = dict(rotary=64, inv_freq=f)
+    check_append(b)
+
+
+# ---- attend: one new token per sequence ----------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_decode_lengths(F, ctx, dtype, dim):
+    lens = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 191, 700, 0]
+    Batch(F, ctx, lens=lens, dim=dim, dtype=dtype, page=32).check_attend()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (5, 5), (8, 1), (9, 1), (40, 8), (16, 1), (17, 1), (48, 2), (71, 1)])
+def test_decode_head_layouts(F, ctx, heads, kv_heads):
+    Batch(F, ctx, lens=[129, 5, 1, 260], heads=heads, kv_heads=kv_heads, page=64).check_attend()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_pages(F, ctx, page, dtype):
+    Batch(F, ctx, lens=[600, 256, 257, 40, 1], page=page, dtype=dtype).check_attend()
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 65, 200, 10 ** 6])
+def test_decode_window(F, ctx, window):
+    Batch(F, ctx, lens=[300, 64, 65, 1, 201], page=16).check_attend(window=window)
+
+
+def test_decode_long_and_short_together(F, ctx):
+    Batch(F, ctx, lens=[20000, 1, 3, 7001, 64, 0, 12345], heads=4, kv_heads=1, page=64, base=1e6).check_attend()
+
+
+@pytest.mark.parametrize("seqs", [200, 777])
+def test_decode_many_sequences(F, ctx, seqs):
+    Batch(F, ctx, lens=[(37 * i) % 150 for i in range(seqs)], heads=2, kv_heads=1, dim=64, page=16).check_attend()
+
+
+def test_decode_rotations(F, ctx):
+    for rotary, inter in [(0, False), (64, False), (64, True), (128, True), (16, False)]:
+        Batch(F, ctx, lens=[90, 4000], rotary=rotary, interleaved=inter, page=64, base=1e6).check_attend()
+
+
+def test_decode_absent_pages_are_not_seen(F, ctx):
+    b = Batch(F, ctx, lens=[200, 100, 16])
+    b.table[0, 0:3] = -1                                       # given back
+    b.table[0, 7] = 2 ** 31 - 1
+    b.table[1, :] = -7                                         # nothing left: zeros
+    b.seqs.page_table.copy_(b.table)
+    y = b.check_attend()
+    assert (y[1] == 0).all()
+
+
+def test_decode_length_past_the_table_reads_only_the_table(F, ctx):
+    b = Batch(F, ctx, lens=[64, 48], spare_cols=0)
+    for n in (2 ** 31 - 1, 65, 10 ** 6):
+        b.lens[0] = n
+        b.seqs.lens.copy_(torch.tensor(b.lens, dtype=torch.int32))
+        b.check_attend()
+    b.lens[0], b.rope, b.rope_ref = -(2 ** 31), None, dict(rotary=0)
+    b.seqs.lens.copy_(torch.tensor(b.lens, dtype=torch.int32))
+    assert (b.check_attend()[0] == 0).all()
+
+
+def test_decode_large_and_tiny_scores(F, ctx):
+    for scale in (1e-6, 3.0, 60.0, -1.0):
+        Batch(F, ctx, lens=[333, 64], dtype=HF).check_attend(scale=scale)
+        Batch(F, ctx, lens=[333, 64], dtype=BF).check_attend(scale=scale)
+
+
+def test_decode_weights_over_many_magnitudes(F, ctx):
+    """One key far above thousands of small ones whose sum still counts: small weights must not be lost."""
+    b = Batch(F, ctx, lens=[6000], heads=1, kv_heads=1, rotary=0, dtype=HF, page=64)
+    b.q.zero_()
+    b.q[0, 0] = 1.0
+    K = b.cache.k
+    K[torch.isfinite(K)] = 0.0
+    pg = int(b.table[0, 10])
+    K[pg, 0, 5, 0] = 13.0                                      # e^13 = 4.4e5 against 6000 ones
+    V = b.cache.v
+    V[torch.isfinite(V)] = 1.0
+    V[pg, 0, 5] = 0.0
+    b.check_attend(scale=1.0)
+
+
+# ---- attend: several new tokens ---------------------------------------------------------------------------
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 8, 2), (128, 5, 1), (256, 4, 2)])
+def test_new_tokens_see_up_to_themselves(F, ctx, out_dtype, dtype, dim, heads, kv_heads):
+    b = Batch(F, ctx, lens=[5, 1, 70, 130, 300, 64], new=[5, 1, 3, 130, 7, 0], dim=dim, heads=heads, kv_heads=kv_heads, dtype=dtype,
+              page=32, pad_rows=2)
+    b.check_attend(out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompts(F, ctx, out_dtype, dtype, dim):
+    b = Batch(F, ctx, lens=[257, 400, 129], new=[257, 130, 1], heads=4, kv_heads=2, dim=dim, dtype=dtype, page=64, pad_rows=1)
+    b.check_attend(out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prompt_pages(F, ctx, page, dtype):
+    Batch(F, ctx, lens=[330, 90], new=[200, 90], heads=2, kv_heads=1, page=page, dtype=dtype).check_attend(out_dtype=BF)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+@pytest.mark.parametrize("window", [1, 5, 64, 100, 129])
+def test_prompt_window(F, ctx, out_dtype, window):
+    Batch(F, ctx, lens=[300, 90, 200], new=[290, 90, 140], heads=2, kv_heads=1, page=16).check_attend(window=window, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (40, 8), (12, 1), (64, 1), (129, 1), (200, 1)])
+def test_prompt_head_layouts(F, ctx, heads, kv_heads):
+    Batch(F, ctx, lens=[70, 150], new=[70, 13], heads=heads, kv_heads=kv_heads, dim=64, page=64).check_attend(out_dtype=BF)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+def test_tokens_below_zero_and_absent_pages(F, ctx, out_dtype):
+    b = Batch(F, ctx, lens=[10, 200, 300, 0], new=[100, 150, 120, 4], heads=4, kv_heads=1, page=32)
+    b.table[1, 1:4] = -1
+    b.table[2, :] = 1 << 30
+    b.seqs.page_table.copy_(b.table)
+    y = b.check_attend(out_dtype=out_dtype)
+    assert (y[:90] == 0).all() and (y[250:370] == 0).all()
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+@pytest.mark.parametrize("new", [[4, 6], [90, 100]])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_what_is_not_finite_reaches_only_the_tokens_that_see_it(F, ctx, out_dtype, new, bad):
+    b = Batch(F, ctx, lens=[130, 150], new=new, heads=4, kv_heads=2, page=16)
+    at = 140                                                   # position in the second sequence, its head 1
+    want, bound, _ = R.attend(b.cache.k, b.cache.v, b.table, b.lens, b.starts, b.q, b.heads, b.rope_ref, out_dtype=out_dtype)
+    pg = int(b.table[1, at // 16])
+    b.cache.v[pg, 1, at % 16, 3] = bad
+    b.cache.k[pg, 1, at % 16, 9] = float("nan") if bad != bad else b.cache.k[pg, 1, at % 16, 9]
+    y = b.cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=out_dtype).double().cpu().reshape(b.tokens, 4, 128)
+    pos = torch.tensor([n - m + j for n, m in zip(b.lens, new) for j in range(m)])
+    seq = torch.tensor([i for i, m in enumerate(new) for _ in range(m)])
+    sees = (seq == 1) & (pos >= at)
+    off = (y - want.reshape(b.tokens, 4, 128)).abs()
+    fine = off <= bound.reshape(b.tokens, 4, 128)
+    assert fine[~sees].all() and fine[:, :2].all()
+    assert not torch.isfinite(y[sees][:, 2:, 3]).any()
+    if bad == bad:                                             # only element 3 of the value was touched
+        keep = [i for i in range(128) if i != 3]
+        assert fine[sees][:, 2:][..., keep].all()
+
+
+def test_value_outside_the_window_does_not_leak(F, ctx):
+    b = Batch(F, ctx, lens=[200, 200], new=[1, 40], heads=4, kv_heads=1, page=16)
+    for i in range(2):
+        b.cache.v[int(b.table[i, 70 // 16]), 0, 70 % 16] = float("inf")
+        b.cache.k[int(b.table[i, 71 // 16]), 0, 71 % 16] = float("nan")
+    b.check_attend(window=80)
+
+
+# ---- entry points in use ------------------------------------------------------------------------------------
+def test_prompt_then_tokens_equals_the_whole_prompt(F, ctx):
+    """A prompt in two chunks and three single tokens give what one pass over all of it gives."""
+    T = 150
+    b = Batch(F, ctx, lens=[T], new=[T], heads=4, kv_heads=2, page=32, fill=False)
+    b.cache.append(b.seqs, b.k, b.v, rope=b.rope)
+    whole = b.cache.attend(b.seqs, b.q, rope=b.rope)
+    b.check_attend()
+    k_all, v_all = b.cache.k.clone(), b.cache.v.clone()
+    b.cache.k.fill_(float("nan"))
+    b.cache.v.fill_(float("nan"))
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    rows, at = [], 0
+    for n in (100, 47, 1, 1, 1):
+        s = F.KVSeqs(b.seqs.page_table, dev([at + n]), None if n == 1 else dev([0, n]))
+        sl = slice(at, at + n)
+        b.cache.append(s, b.k[sl], b.v[sl], rope=b.rope)
+        rows.append(b.cache.attend(s, b.q[sl], rope=b.rope))
+        at += n
+    assert torch.equal(b.cache.k.view(torch.int16), k_all.view(torch.int16)) and torch.equal(b.cache.v.view(torch.int16), v_all.view(torch.int16))
+    want, bound, _ = R.attend(b.cache.k, b.cache.v, b.table, b.lens, b.starts, b.q, 4, b.rope_ref)
+    assert ((torch.cat(rows).double().cpu() - want).abs() <= bound).all()
+    assert ((torch.cat(rows) - whole).double().cpu().abs() <= 2 * bound).all()
+
+
+@pytest.mark.parametrize("lens,new,out_dtype", [([5000, 64, 1, 1999], None, torch.float32), ([300, 700], [150, 260], BF), ([900, 70], [5, 5], BF)])
+def test_the_same_call_gives_the_same_bits(F, ctx, lens, new, out_dtype):
+    b = Batch(F, ctx, lens=lens, new=new, heads=8, kv_heads=2, page=16)
+    first = b.cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=out_dtype)
+    for _ in range(3):
+        assert torch.equal(b.cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=out_dtype), first)
+
+
+def test_captured_step_follows_lengths_and_pages(F, ctx):
+    """Append + attend captured once; replayed while the lengths grow and the page table changes under it."""
+    b = Batch(F, ctx, lens=[30, 100, 63], heads=8, kv_heads=2, page=16, spare_cols=3)
+    n_pages = b.cache.k.shape[0]
+    more = F.KVCache.empty(ctx, n_pages + 6, 16, 2, 128)
+    more.k[:n_pages], more.v[:n_pages] = b.cache.k, b.cache.v
+    b.cache = more
+    out = torch.empty((3, 8 * 128), device="cuda")
+
+    def step():
+        b.seqs.lens.add_(1)
+        b.cache.append(b.seqs, b.k, b.v, rope=b.rope)
+        b.cache.attend(b.seqs, b.q, rope=b.rope, out=out)
+
+    spare = n_pages
+    def grow():
+        nonlocal spare
+        for i in range(3):
+            b.lens[i] += 1
+            c = (b.lens[i] - 1) // 16
+            if int(b.table[i, c]) < 0:
+                b.table[i, c] = spare
+                spare += 1
+        b.seqs.page_table.copy_(b.table)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ctx.use_torch_stream()
+        grow()
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ctx.use_torch_stream()
+        step()
+    ctx.use_torch_stream()
+    for k in range(20):
+        b.qkv.copy_(torch.randn(b.qkv.shape, generator=torch.Generator().manual_seed(100 + k)))
+        grow()
+        g.replay()
+        if k % 6 == 1:
+            torch.cuda.synchronize()
+            want, bound, _ = R.attend(b.cache.k, b.cache.v, b.table, b.lens, None, b.q, 8, b.rope_ref)
+            assert ((out.double().cpu() - want).abs() <= bound).all()
+    assert b.seqs.lens.tolist() == b.lens
+
+
+def test_two_contexts_on_two_streams(F):
+    """Graphs of two contexts replayed at the same time: each has a workspace of its own."""
+    runs = []
+    for i in range(2):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            c = F.Context(0)
+            b = Batch(F, c, lens=[3000 + 500 * i, 700, 64], heads=8, kv_heads=1, page=64, seed=i)
+            out = torch.empty((3, 8 * 128), device="cuda")
+            want = b.cache.attend(b.seqs, b.q, rope=b.rope, out=out).clone()
+            st.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                for _ in range(20):
+                    b.cache.attend(b.seqs, b.q, rope=b.rope, out=out)
+            runs.append((st, c, b, out, want, g))
+    for _ in range(10):
+        for st, _, _, out, _, g in runs:
+            with torch.cuda.stream(st):
+                out.zero_()
+                g.replay()
+    torch.cuda.synchronize()
+    for _, c, _, out, want, g in runs:
+        assert torch.equal(out, want)
+    for r in runs:
+        r[1].close()
+
+
+def test_context_with_a_stream_of_its_own(F):
+    c = F.Context(0, stream=None)
+    b = Batch(F, c, lens=[100, 9], new=[4, 9], fill=False)
+    b.cache.k.zero_(), b.cache.v.zero_()
+    torch.cuda.synchronize()
+    b.cache.append(b.seqs, b.k, b.v, rope=b.rope)
+    y = b.cache.attend(b.seqs, b.q, rope=b.rope)
+    c.sync()
+    want, bound, _ = R.attend(b.cache.k, b.cache.v, b.table, b.lens, b.starts, b.q, b.heads, b.rope_ref)
+    assert ((y.double().cpu() - want).abs() <= bound).all()
+    c.close()
+
+
+def test_operands_that_are_not_dense(F, ctx):
+    """3-D views, odd strides and offsets: taken in place or copied, never misread."""
+    b = Batch(F, ctx, lens=[50, 60, 70], page=32)
+    want = b.cache.attend(b.seqs, b.q, rope=b.rope)
+    wide = torch.full((3, b.heads * 128 + 7), 3.0, device="cuda")
+    wide[:, 5:5 + b.heads * 128] = b.q
+    odd = wide[:, 5:5 + b.heads * 128]                          # neither aligned nor a stride of four
+    assert torch.equal(b.cache.attend(b.seqs, odd, rope=b.rope), want)
+    assert torch.equal(b.cache.attend(b.seqs, b.q.reshape(3, b.heads, 128), rope=b.rope), want)
+    apart = torch.zeros((3, b.heads, 2, 128), device="cuda")
+    apart[:, :, 0] = b.q.reshape(3, b.heads, 128)
+    assert torch.equal(b.cache.attend(b.seqs, apart[:, :, 0], rope=b.rope), want)
+    slot = torch.full((3, b.heads * 128 + 64), 5.0, device="cuda")
+    b.cache.attend(b.seqs, b.q, rope=b.rope, out=slot[:, 32:32 + b.heads * 128])
+    assert torch.equal(slot[:, 32:32 + b.heads * 128], want) and (slot[:, :32] == 5).all() and (slot[:, 32 + b.heads * 128:] == 5).all()
+
+
+def test_no_tokens_and_no_sequences(F, ctx):
+    b = Batch(F, ctx, lens=[20], new=[0])
+    assert b.cache.attend(b.seqs, b.q, rope=b.rope).shape == (0, b.heads * b.dim)
+    b.cache.append(b.seqs, b.k, b.v)
+    s = F.KVSeqs(torch.empty((0, 4), dtype=torch.int32, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"))
+    b.cache.append(s, b.k, b.v)
+    assert b.cache.attend(s, b.q).shape[0] == 0
+
+
+def test_starts_that_make_no_sense_stay_inside_the_activations(F, ctx):
+    b = Batch(F, ctx, lens=[40, 40, 40], new=[10, 10, 10])
+    for starts in ([0, 50, 20, 30], [-9, 10, 2 ** 31 - 1, 5], [30, 20, 10, 0], [5, 5, 5, 5]):
+        b.seqs.starts.copy_(torch.tensor(starts, dtype=torch.int32))
+        for ty in (torch.float32, BF):
+            b.cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=ty)
+        b.cache.append(b.seqs, b.k, b.v, rope=b.rope)
+    torch.cuda.synchronize()
+    assert b.cache.ctx.launches() > 0
+
+
+def test_a_cache_past_32_bit_offsets(F, ctx):
+    """Pages whose element offsets pass 2^31 (and byte offsets 2^32)."""
+    n_pages = (1 << 31) // (8 * 64 * 128) + 8
+    cache = F.KVCache.empty(ctx, n_pages, 64, 8, 128)
+    lens = [200, 65]
+    table = torch.tensor([[n_pages - 1, 0, n_pages - 3, 5, -1], [n_pages - 2, n_pages - 4, -1, -1, -1]], dtype=torch.int32)
+    b = Batch(F, ctx, lens=lens, new=lens, heads=8, kv_heads=8, page=64, fill=False)
+    b.cache, b.table = cache, table
+    b.seqs = F.KVSeqs(table.cuda(), b.seqs.lens, b.seqs.starts)
+    cache.append(b.seqs, b.k, b.v, rope=b.rope)
+    ids = sorted(set(int(x) for x in table.flatten() if x >= 0))
+    small = torch.full_like(table, -1)
+    for i, p in enumerate(ids):
+        small[table == p] = i
+    kc, vc = cache.k[ids], cache.v[ids]
+    for ty in (torch.float32, BF):
+        y = cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=ty).double().cpu()
+        want, bound, _ = R.attend(kc, vc, small, lens, b.starts, b.q, 8, b.rope_ref, out_dtype=ty)
+        assert ((y - want).abs() <= bound).all()
+
+
+# ---- refusals -----------------------------------------------------------------------------------------------
+def test_refusals(F, ctx):
+    b = Batch(F, ctx, lens=[20, 30])
+    cu = lambda *s, **k: torch.zeros(s, device="cuda", **k)
+    with pytest.raises(TypeError):
+        F.KVCache(ctx, cu(2, 2, 16, 128), cu(2, 2, 16, 128))                       # f32
+    with pytest.raises(TypeError):
+        F.KVCache(ctx, cu(2, 2, 16, 128, dtype=BF), cu(2, 2, 16, 128, dtype=HF))
+    with pytest.raises(ValueError):
+        F.KVCache(ctx, cu(2, 2, 128, 16, dtype=BF).transpose(2, 3), cu(2, 2, 128, 16, dtype=BF).transpose(2, 3))
+    for shape in ((2, 2, 24, 128), (2, 2, 16, 96), (2, 2, 512, 64)):
+        c = F.KVCache(ctx, cu(*shape, dtype=BF), cu(*shape, dtype=BF))
+        with pytest.raises(F.FerricError) as e:
+            c.attend(b.seqs, cu(2, 4 * shape[3]))
+        assert e.value.status == 3
+    with pytest.raises(F.FerricError) as e:
+        b.cache.attend(b.seqs, cu(2, 3 * 128))                                     # 3 heads over 2
+    assert e.value.status == 3
+    with pytest.raises(F.FerricError) as e:
+        b.cache.attend(b.seqs, cu(3, 8 * 128))                                     # 3 tokens, 2 sequences
+    assert e.value.status == 3 and "one token per sequence" in str(e.value)
+    with pytest.raises(ValueError):
+        b.cache.append(b.seqs, b.k, b.q)
+    with pytest.raises(ValueError):
+        b.cache.attend(b.seqs, cu(2, 8 * 128 + 4))
+    with pytest.raises(TypeError):
+        b.cache.attend(b.seqs, b.q.half())
+    with pytest.raises(TypeError):
+        b.cache.attend(b.seqs, b.q, out_dtype=HF)
+    with pytest.raises(ValueError):
+        b.cache.attend(b.seqs, b.q, window=-1)
+    with pytest.raises(ValueError):
+        b.cache.attend(b.seqs, b.q, scale=0.0)
+    with pytest.raises(F.FerricError):
+        b.cache.attend(b.seqs, b.q, scale=float("nan"))
+    with pytest.raises(F.FerricError):
+        b.cache.attend(b.seqs, b.q, out=cu(2, 8 * 128 + 1)[:, 1:])                 # not 16-byte aligned
+    with pytest.raises(F.FerricError):
+        F.Rope(ctx, 24)
+    with pytest.raises(F.FerricError):
+        F.Rope(ctx, 64, base=-1.0)
+    with pytest.raises(ValueError):
+        F.Rope(ctx, 64, inv_freq=[1.0] * 31)
+    with pytest.raises(F.FerricError):
+        F.Rope(ctx, 32, inv_freq=[float("inf")] * 16)
+    with pytest.raises(F.FerricError):
+        b.cache.attend(b.seqs, b.q, rope=F.Rope(ctx, 256))                         # heads have 128
+    with pytest.raises(TypeError):
+        F.KVSeqs(b.seqs.page_table.long(), b.seqs.lens)
+    with pytest.raises(ValueError):
+        F.KVSeqs(b.seqs.page_table, b.seqs.lens[:1])
+    b.check_attend()                                                              # and the context still works

@@ -1,0 +1,192 @@
+"""The cache operators without a GPU: the index arithmetic the kernels compile, driven through a g++ shim, and the C ABI's
+refusals (the context is checked last, so every other refusal shows without a device; no pointer is followed)."""
+import ctypes as C
+import os
+import random
+import subprocess
+import tempfile
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+I32 = 2 ** 31
+
+
+@pytest.fixture(scope="module")
+def shim():
+    out = os.path.join(tempfile.mkdtemp(prefix="ferric_kv_shim_"), "kv_shim.so")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-fsanitize=signed-integer-overflow", "-fno-sanitize-recover=all", "-shared", "-fPIC", "-o", out,
+                           os.path.join(HERE, "cpu", "kv_shim.cpp")])
+    lib = C.CDLL(out)
+    lib.shim_offset.restype = C.c_longlong
+    lib.shim_offset.argtypes = [C.c_int] * 4 + [C.c_longlong, C.c_void_p, C.c_longlong] + [C.c_int] * 5
+    return lib
+
+
+def ints(v):
+    return (C.c_int * len(v))(*v)
+
+
+def test_spans_stay_inside_the_activations(shim):
+    r = random.Random(3)
+    out = (C.c_int * 4)()
+    for _ in range(3000):
+        n, tokens = r.randint(1, 6), r.randint(0, 40)
+        starts = [r.choice([r.randint(-50, 50), -I32, I32 - 1]) for _ in range(n + 1)]
+        lens = [r.choice([r.randint(-5, 100), -I32, I32 - 1]) for _ in range(n)]
+        for i in range(n):
+            shim.shim_span(ints(lens), ints(starts), n, tokens, i, out)
+            first, m = out[0], out[1]
+            assert m >= 0 and first >= 0 and (m == 0 or first + m <= tokens)
+            if m:
+                assert out[3] == max(-I32, lens[i] - 1)
+        for t in range(tokens):
+            s = shim.shim_seq_of(ints(starts), n, tokens, t)
+            assert s == -1 or (0 <= s < n and starts[s] <= t < starts[s + 1])
+
+
+def test_rows_find_their_sequence(shim):
+    r = random.Random(4)
+    for _ in range(300):
+        n = r.randint(1, 20)
+        starts = [r.randint(0, 3)]
+        for _ in range(n):
+            starts.append(starts[-1] + r.choice([0, 0, 1, 2, 7]))
+        for t in range(starts[-1] + 4):
+            want = [i for i in range(n) if starts[i] <= t < starts[i + 1]]
+            assert shim.shim_seq_of(ints(starts), n, starts[-1] + 4, t) == (want[0] if want else -1)
+    assert shim.shim_seq_of(None, 3, 5, 2) == 2 and shim.shim_seq_of(None, 3, 5, 3) == -1
+
+
+def test_offsets_are_inside_the_cache_or_absent(shim):
+    r = random.Random(5)
+    for _ in range(4000):
+        shift, heads, dim, n_pages = r.randint(4, 8), r.randint(1, 9), r.choice([64, 128, 256]), r.choice([0, 1, 7, I32 - 1, 200000])
+        stride = heads * dim << shift
+        stride += r.choice([0, 8, stride])
+        cols, n = r.randint(1, 6), r.randint(1, 3)
+        ts = cols + r.randint(0, 3)
+        table = ints([r.choice([0, 1, n_pages - 1, n_pages, -1, -I32, I32 - 1, r.randrange(max(1, n_pages))]) for _ in range(n * ts)])
+        seq, h = r.randrange(n), r.randrange(heads)
+        pos = r.choice([0, (cols << shift) - 1, cols << shift, -1, -I32, I32 - 1, r.randrange(cols << shift)])
+        off = shim.shim_offset(n_pages, heads, shift, dim, stride, table, ts, cols, n, seq, h, pos)
+        if 0 <= pos < cols << shift and 0 <= table[seq * ts + (pos >> shift)] < n_pages:
+            assert off == table[seq * ts + (pos >> shift)] * stride + ((h << shift) + pos % (1 << shift)) * dim
+            assert 0 <= off <= n_pages * stride - dim
+        else:
+            assert off == -1
+
+
+def test_seen_keys(shim):
+    out = (C.c_int * 2)()
+    for shift, cols in [(4, 3), (8, 1), (4, 1 << 26), (8, 1 << 22), (8, 0)]:
+        for pos in (-I32, -1, 0, 1, 15, 47, 48, 300, I32 - 1):
+            for window in (0, 1, 2, 16, I32 - 1):
+                shim.shim_seen(shift, cols, pos, window, out)
+                cap = cols << shift
+                assert out[1] == min(cap, max(0, pos + 1))
+                assert out[0] == (max(0, pos - window + 1) if window else 0)
+
+
+# ---- the C ABI ----------------------------------------------------------------------------------------
+P = 1 << 20          # an aligned address that is never followed
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from ferric_b200 import build, _lib
+    build.build()
+    return _lib.load()
+
+
+def cache(**kw):
+    from ferric_b200 import _lib
+    d = dict(k_dev=P, v_dev=P, ggml_type=30, n_pages=10, page_size=16, n_heads=2, head_dim=128, page_stride=0)
+    d.update(kw)
+    return _lib.KvCache(**d)
+
+
+def seqs(**kw):
+    from ferric_b200 import _lib
+    d = dict(page_table_dev=P, n_seqs=3, max_pages=4, table_stride=0, lens_dev=P, starts_dev=None)
+    d.update(kw)
+    return _lib.KvSeqs(**d)
+
+
+def call(lib, fn, c=None, s=None, n=3, **kw):
+    c, s = cache() if c is None else c, seqs() if s is None else s
+    cp, sp = (C.byref(c) if c else None), (C.byref(s) if s else None)
+    if fn == "append":
+        d = dict(k=P, ldk=0, v=P, ldv=0)
+        d.update(kw)
+        rc = lib.ferric_cuda_kv_append(None, cp, sp, None, d["k"], d["ldk"], d["v"], d["ldv"], n)
+    else:
+        d = dict(q=P, ldq=0, heads=8, scale=0.0, window=0, out=P, ty=0, ldo=0)
+        d.update(kw)
+        rc = lib.ferric_cuda_kv_attend(None, cp, sp, None, d["q"], d["ldq"], n, d["heads"], d["scale"], d["window"], d["out"], d["ty"], d["ldo"])
+    return rc, lib.ferric_cuda_last_error().decode()
+
+
+@pytest.mark.parametrize("fn", ["append", "attend"])
+def test_a_sound_call_without_a_context(lib, fn):
+    assert call(lib, fn) == (1, "NULL context")
+
+
+@pytest.mark.parametrize("fn", ["append", "attend"])
+@pytest.mark.parametrize("bad,rc,word", [
+    (dict(ggml_type=0), 2, "f16 or bf16"), (dict(ggml_type=12), 2, "f16 or bf16"), (dict(head_dim=96), 3, "head_dim"), (dict(head_dim=0), 3, "head_dim"),
+    (dict(page_size=24), 3, "page_size"), (dict(page_size=8), 3, "page_size"), (dict(page_size=512), 3, "page_size"), (dict(n_heads=0), 3, "heads"),
+    (dict(page_stride=4096 - 8), 3, "page_stride"), (dict(page_stride=4100), 3, "page_stride"), (dict(n_pages=I32), 3, "pages"),
+    (dict(n_pages=I32 - 1, page_stride=1 << 40), 3, "pages"), (dict(k_dev=None), 1, "NULL cache"), (dict(v_dev=P + 8), 1, "aligned"),
+])
+def test_bad_caches(lib, fn, bad, rc, word):
+    got, msg = call(lib, fn, c=cache(**bad))
+    assert got == rc and word in msg
+
+
+@pytest.mark.parametrize("fn", ["append", "attend"])
+@pytest.mark.parametrize("bad,n,rc,word", [
+    (dict(table_stride=3), 3, 3, "table_stride"), (dict(), 4, 3, "one token per sequence"), (dict(lens_dev=None), 3, 1, "NULL lengths"),
+    (dict(page_table_dev=None), 3, 1, "page table"), (dict(lens_dev=P + 2), 3, 1, "aligned"), (dict(max_pages=I32), 3, 3, "pages"), (dict(max_pages=(1 << 26) + 1), 3, 3, "2^30"),
+    (dict(n_seqs=1 << 21), 1 << 21, 3, "sequences"), (dict(starts_dev=P), I32, 3, "tokens"),
+])
+def test_bad_sequence_tables(lib, fn, bad, n, rc, word):
+    got, msg = call(lib, fn, s=seqs(**bad), n=n)
+    assert got == rc and word in msg
+
+
+def test_bad_operands(lib):
+    for kw, rc in [(dict(k=None), 1), (dict(v=P + 4), 1), (dict(ldk=252), 3), (dict(ldv=258), 3), (dict(ldk=1 << 62), 3)]:
+        assert call(lib, "append", **kw)[0] == rc
+    for kw, rc in [(dict(q=None), 1), (dict(out=None), 1), (dict(out=P + 8), 1), (dict(q=P + 4), 1), (dict(ldq=1020), 3), (dict(ldo=1020), 3),
+                   (dict(heads=3), 3), (dict(heads=0), 3), (dict(ty=1), 2), (dict(ty=30, ldo=1028), 3), (dict(scale=float("nan")), 1),
+                   (dict(scale=float("inf")), 1), (dict(heads=1 << 20), 3)]:
+        assert call(lib, "attend", **kw)[0] == rc, kw
+    assert call(lib, "attend", ty=30, ldo=1032)[1] == "NULL context"
+    h = C.c_void_p()
+    assert lib.ferric_cuda_rope_create(None, 64, 1e4, None, 0, C.byref(h)) == 1
+    lib.ferric_cuda_rope_free(None)
+    assert lib.ferric_cuda_attend_reserve(None) == 1
+    assert call(lib, "append", c=False)[1] == "NULL cache" and call(lib, "attend", s=False)[1] == "NULL sequence table"
+
+
+def test_the_64_bit_evaluation_against_differences():
+    """The tests' own reference: rotation keeps lengths and composes, attention is the weighted mean of its definition."""
+    import torch
+
+    import kv_ref as R
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn((3, 2, 64), generator=g, dtype=torch.float64)
+    for inter in (False, True):
+        y = R.rotate(x, torch.tensor([5, 70000, 9]), 32, interleaved=inter)
+        assert torch.allclose(y.norm(dim=-1), x.norm(dim=-1)) and torch.equal(y[..., 32:], x[..., 32:])
+        z = R.rotate(R.rotate(x, torch.tensor([3, 4, 5]), 64, interleaved=inter), torch.tensor([4, 4, 4]), 64, interleaved=inter)
+        assert torch.allclose(z, R.rotate(x, torch.tensor([7, 8, 9]), 64, interleaved=inter))
+    kc = torch.randn((3, 1, 16, 64), generator=g).to(torch.bfloat16)
+    vc = torch.randn((3, 1, 16, 64), generator=g).to(torch.bfloat16)
+    q = torch.randn((2, 128), generator=g)
+    out, bound, mine = R.attend(kc, vc, torch.tensor([[2, 0]]), [20], [0, 2], q, 2, dict(rotary=0))
+    k = torch.cat([kc[2, 0], kc[0, 0]])[:20].double()
+    v = torch.cat([vc[2, 0], vc[0, 0]])[:20].double()
+    w = torch.exp(q.double()[0, 64:] @ k[:19].T / 8)
+    assert mine.all() and torch.allclose(out[0, 64:], (w @ v[:19]) / w.sum()) and (bound > 0).all()
