@@ -219,7 +219,10 @@ struct AttendArgs {
     float scale = 0.0f;
     int window = 0;                  // keys a token sees at most; 0: all up to its own
 };
-int32_t launch_attend(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a,
+// `ws` holds attend_ws_bytes() bytes, the first attend_ticket_bytes() of them zero between launches.
+size_t attend_ws_bytes(int sm_count);
+size_t attend_ticket_bytes();
+int32_t launch_attend(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a, void* ws,
                       const GemvTuning& tune, int* launches);
 
 // Synchronise the stream and fetch-and-clear the code a GEMM CTA left when one of its bounded waits ran out.

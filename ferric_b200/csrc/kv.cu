@@ -231,6 +231,24 @@ int32_t ferric_cuda_attend_reserve(ferric_cuda_ctx* ctx)
         set_last_error("NULL context");
         return kErrInvalidArg;
     }
+    if (ctx->attend_ws) return kOk;
+    DeviceGuard guard(ctx->device);
+    if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    FERRIC_CUDA_TRY(cudaStreamIsCapturing(ctx->stream, &cap));
+    if (cap != cudaStreamCaptureStatusNone) {
+        set_last_error("the attention's workspace is not allocated yet: call ferric_cuda_attend_reserve (or attend once) before capturing");
+        return kErrInvalidArg;
+    }
+    void* ws = nullptr;
+    FERRIC_CUDA_TRY(cudaMalloc(&ws, attend_ws_bytes(ctx->tune.sm_count)));
+    cudaError_t e = cudaMemsetAsync(ws, 0, attend_ticket_bytes(), ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+    if (e != cudaSuccess) {
+        cudaFree(ws);
+        return cuda_fail(e, "attend_reserve");
+    }
+    ctx->attend_ws = ws;
     return kOk;
 }
 
@@ -284,9 +302,10 @@ int32_t ferric_cuda_kv_attend(ferric_cuda_ctx* ctx, const ferric_kv_cache* cache
     a.window = window > (size_t)INT32_MAX ? 0 : (int)window;   // a window past every position hides nothing
     DeviceGuard guard(ctx->device);
     if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
+    if ((rc = ferric_cuda_attend_reserve(ctx)) != kOk) return rc;
     int launched = 0;
-    rc = launch_attend(ctx->stream, c, s, r, a, ctx->tune, &launched);
-    ctx->launches += launched;
+    rc = launch_attend(ctx->stream, c, s, r, a, ctx->attend_ws, ctx->tune, &launched);
+    if (rc == kOk) ctx->launches += launched;
     return rc;
 }
 

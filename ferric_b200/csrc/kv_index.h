@@ -97,4 +97,56 @@ FERRIC_KV_HD int kv_seen_hi(const KvCacheView& c, const KvSeqsView& s, int pos)
     return (int)(h < cap ? h : cap);
 }
 
+// ---- the attention's work split ---------------------------------------------------------------------------------------
+// The query rows of a sequence and key-value head are its (token, query head of the group) pairs, token-major; a block is
+// `rb` of them, against key tiles of kAttendTile positions.  All tiles of all blocks -- sequence by sequence, head by head,
+// block by block -- form one line that is cut evenly over the CTAs, wherever blocks begin and end: the lengths decide on the
+// device, so a captured launch stays balanced when they change.
+constexpr int kAttendTile = 64;
+struct AttendBlock {
+    int r0, rows;      // query rows [r0, r0 + rows) of the sequence
+    int j0, j1;        // new tokens of the first and the last row
+    int lo, hi;        // keys that any of the rows sees
+    int t0, tiles;     // key tiles [t0, t0 + tiles); a block that sees nothing has one, with every key masked
+};
+FERRIC_KV_HD int attend_blocks(const KvSpan& p, int group, int rb) { return (p.n * group + rb - 1) / rb; }
+FERRIC_KV_HD AttendBlock attend_block(const KvCacheView& c, const KvSeqsView& s, const KvSpan& p, int group, int rb, int window, int b)
+{
+    AttendBlock k;
+    k.r0 = b * rb;
+    k.rows = kv_min(p.n * group - k.r0, rb);
+    k.j0 = k.r0 / group;
+    k.j1 = (k.r0 + k.rows - 1) / group;
+    k.lo = kv_seen_lo(p.pos(k.j0), window);
+    k.hi = kv_seen_hi(c, s, p.pos(k.j1));
+    k.t0 = k.lo / kAttendTile;
+    k.tiles = (k.hi + kAttendTile - 1) / kAttendTile - k.t0;
+    if (k.hi <= k.lo) {
+        k.lo = k.hi = k.t0 = 0;
+        k.tiles = 1;
+    }
+    return k;
+}
+// Tiles of one head of a sequence.
+FERRIC_KV_HD long long attend_seq_tiles(const KvCacheView& c, const KvSeqsView& s, const KvSpan& p, int group, int rb, int window)
+{
+    const int nb = attend_blocks(p, group, rb);
+    if (nb == 0) return 0;
+    if (p.n == 1) return (long long)nb * attend_block(c, s, p, group, rb, window, 0).tiles;
+    long long t = 0;
+    for (int b = 0; b < nb; b++) t += attend_block(c, s, p, group, rb, window, b).tiles;
+    return t;
+}
+// `total` tiles over `parts` CTAs: part i starts at attend_cut(i), and tile x is attend_part_of(x)'s.
+FERRIC_KV_HD long long attend_cut(long long total, int parts, int i)
+{
+    const long long q = total / parts, r = total % parts;
+    return i * q + (i < r ? i : r);
+}
+FERRIC_KV_HD int attend_part_of(long long total, int parts, long long x)
+{
+    const long long q = total / parts, r = total % parts;
+    return (int)(x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q);
+}
+
 }  // namespace ferric

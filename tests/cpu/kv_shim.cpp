@@ -45,4 +45,25 @@ void shim_seen(int page_shift, int cols, int pos, int window, int* lo_hi)
     lo_hi[0] = kv_seen_lo(pos, window);
     lo_hi[1] = kv_seen_hi(c, seqs(nullptr, 0, cols, nullptr, nullptr, 0, 0), pos);
 }
+// blocks of one sequence: out[b] = {r0, rows, j0, j1, lo, hi, t0, tiles}; returns their number
+int shim_blocks(int page_shift, int cols, int first, int n, int len, int group, int rb, int window, int* out, int cap, long long* tiles)
+{
+    KvCacheView c;
+    c.page_shift = page_shift;
+    const KvSeqsView s = seqs(nullptr, 0, cols, nullptr, nullptr, 1, first + n);
+    KvSpan p;
+    p.first = first;
+    p.n = n;
+    p.len = len;
+    const int nb = attend_blocks(p, group, rb);
+    for (int b = 0; b < nb && b < cap; b++) {
+        const AttendBlock k = attend_block(c, s, p, group, rb, window, b);
+        const int v[8] = {k.r0, k.rows, k.j0, k.j1, k.lo, k.hi, k.t0, k.tiles};
+        for (int i = 0; i < 8; i++) out[8 * b + i] = v[i];
+    }
+    *tiles = attend_seq_tiles(c, s, p, group, rb, window);
+    return nb;
+}
+long long shim_cut(long long total, int parts, int i) { return attend_cut(total, parts, i); }
+int shim_part_of(long long total, int parts, long long x) { return attend_part_of(total, parts, x); }
 }

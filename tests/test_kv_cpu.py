@@ -18,7 +18,9 @@ def shim():
     subprocess.check_call(["g++", "-std=c++17", "-O1", "-fsanitize=signed-integer-overflow", "-fno-sanitize-recover=all", "-shared", "-fPIC", "-o", out,
                            os.path.join(HERE, "cpu", "kv_shim.cpp")])
     lib = C.CDLL(out)
-    lib.shim_offset.restype = C.c_longlong
+    lib.shim_offset.restype = lib.shim_cut.restype = C.c_longlong
+    lib.shim_cut.argtypes = [C.c_longlong, C.c_int, C.c_int]
+    lib.shim_part_of.argtypes = [C.c_longlong, C.c_int, C.c_longlong]
     lib.shim_offset.argtypes = [C.c_int] * 4 + [C.c_longlong, C.c_void_p, C.c_longlong] + [C.c_int] * 5
     return lib
 
@@ -86,6 +88,42 @@ def test_seen_keys(shim):
                 cap = cols << shift
                 assert out[1] == min(cap, max(0, pos + 1))
                 assert out[0] == (max(0, pos - window + 1) if window else 0)
+
+
+def test_blocks_cover_every_row_and_every_key_it_sees(shim):
+    r = random.Random(6)
+    out, tiles = (C.c_int * (8 * 4096))(), C.c_longlong()
+    for _ in range(1500):
+        group, rb, n = r.choice([1, 2, 5, 8, 40]), r.choice([8, 16, 32, 64]), r.choice([0, 1, 1, 2, 5, 33])
+        shift, cols = r.choice([4, 6, 8]), r.choice([0, 1, 7, 100])
+        length = r.choice([0, 1, n, n - 1, 63, 64, 65, 500, 5000, I32 - 1, -I32, -3])
+        window = r.choice([0, 0, 1, 64, 100, I32 - 1])
+        nb = shim.shim_blocks(shift, cols, 0, n, length, group, rb, window, out, 4096, C.byref(tiles))
+        total, row = 0, 0
+        for b in range(nb):
+            r0, rows, j0, j1, lo, hi, t0, nt = out[8 * b:8 * b + 8]
+            assert r0 == row and 1 <= rows <= rb and j0 == r0 // group and j1 == (r0 + rows - 1) // group
+            row += rows
+            total += nt
+            assert nt >= 1 and t0 >= 0
+            for j in (j0, j1):
+                pos = max(-I32, length - n + j)
+                a, z = (max(0, pos - window + 1) if window else 0), min(cols << shift, max(0, pos + 1))
+                assert a >= z or (lo <= a and z <= hi and t0 * 64 <= lo and hi <= (t0 + nt) * 64)
+            assert hi <= cols << shift
+        assert row == n * group and total == tiles.value
+
+
+def test_cuts_are_even_and_found_again(shim):
+    r = random.Random(7)
+    for _ in range(3000):
+        total, parts = r.choice([1, 2, 5, 296, 297, 1000, 10 ** 12]), r.randint(1, 400)
+        parts = min(parts, total)
+        i = r.randrange(parts)
+        a, b = shim.shim_cut(total, parts, i), shim.shim_cut(total, parts, i + 1)
+        assert total // parts <= b - a <= total // parts + 1 and a < b
+        assert shim.shim_part_of(total, parts, a) == i == shim.shim_part_of(total, parts, b - 1)
+        assert shim.shim_cut(total, parts, 0) == 0 and shim.shim_cut(total, parts, parts) == total
 
 
 # ---- the C ABI ----------------------------------------------------------------------------------------
