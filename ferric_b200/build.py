@@ -18,7 +18,7 @@ OBJ = os.path.join(CSRC, "_obj")
 LIB = os.path.join(HERE, "libferric_cuda.so")
 
 SOURCES = ["ffi.cu", "kernels_repack.cu", "kernels_gemv.cu", "kernels_glue.cu", "kernels_gemm.cu", "kernels_gemvtc.cu", "kernels_tpwide.cu", "kernels_kv.cu",
-           "kernels_attend.cu", "gguf.cu", "tp.cu", "kv.cu"]
+           "kernels_attend.cu", "kernels_attend_tc.cu", "gguf.cu", "tp.cu", "kv.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

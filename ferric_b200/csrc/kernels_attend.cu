@@ -651,6 +651,8 @@ EncodeTiledFn encode_tiled_fn()
     return fn;
 }
 
+}  // namespace
+
 // [n_pages][heads][page][dim], read in boxes of 64 elements x up to 64 rows of a page (128-byte swizzle).
 int32_t encode_cache(CUtensorMap* map, const KvCacheView& c, void* base, const void* stand_in)
 {
@@ -674,6 +676,7 @@ int32_t encode_cache(CUtensorMap* map, const KvCacheView& c, void* base, const v
     return kOk;
 }
 
+namespace {
 constexpr size_t kTicketBytes = 8192;   // [2 x SMs]
 
 template <typename T, int D, int WM>
@@ -735,6 +738,7 @@ int32_t launch_attend(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s
                       const GemvTuning& tune, int* launches)
 {
     *launches = 1;
+    if (attend_prompt_eligible(c, s, a)) return launch_attend_prompt(st, c, s, r, a, tune);
     switch (c.dim) {
     case 64: return c.bf16 ? launch_attend_td<__nv_bfloat16, 64>(st, c, s, r, a, ws, tune) : launch_attend_td<__half, 64>(st, c, s, r, a, ws, tune);
     case 128: return c.bf16 ? launch_attend_td<__nv_bfloat16, 128>(st, c, s, r, a, ws, tune) : launch_attend_td<__half, 128>(st, c, s, r, a, ws, tune);

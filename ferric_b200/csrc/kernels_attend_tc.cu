@@ -1,0 +1,505 @@
+// attend_prompt_kernel: attention of many new tokens (prompts and chunks of them), result in bf16, on tcgen05.
+//
+// Bound by the tensor cores (4 head_dim flop per visible pair and query head).  A CTA takes 256 query rows (head_dim 256:
+// 128) of one key-value head -- (token, query head of the group) pairs, so that all heads of the group share the keys it
+// reads -- and walks the keys they see in tiles.  Per tile and 128 rows, a "unit": S = Q K^T into tensor memory; one thread
+// per row takes the softmax step in registers and writes the weights back over S as 16-bit values; O += P V with P read
+// straight from tensor memory and V from shared memory as it lies (rows = keys: the MMA takes it transposed).  There are two
+// S buffers, one per row tile, or alternating over the keys where one row tile fills tensor memory: while one unit is with
+// its softmax warps the other one's products run.
+//
+// The maximum of a row only has to keep 2^(s - m) in range, so it moves -- and O is rescaled, a round trip through registers
+// -- only when the new one exceeds the old one by more than 2^kSlack; the division by the sum makes up for the rest.
+//
+// Rounding: the weights are rounded once to the cache's type (they multiply its values on the tensor cores; 2^-9 of a
+// weight in bf16, as much as the result's own rounding), summed in f32 before that.  q is rounded to f16 for an f16 cache; for
+// a bf16 cache it is split into two bf16 parts, since one alone would move every score by up to 2^-9 of its terms.
+#include <string.h>
+
+#include <type_traits>
+
+#include "kv.cuh"
+#include "tc_common.cuh"
+
+namespace ferric {
+
+int* gemm_status_word();   // device address of the status word shared with the tensor-core products (kernels_gemm.cu)
+int32_t encode_cache(CUtensorMap* map, const KvCacheView& c, void* base, const void* stand_in);   // kernels_attend.cu
+
+template <typename T, int D>
+struct PromptCfg {
+    static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    static constexpr int kParts = kBf16 ? 2 : 1;           // 16-bit parts of q
+    static constexpr int kTilesQ = D == 256 ? 1 : 2;       // row tiles of 128
+    static constexpr int kRows = 128 * kTilesQ;
+    static constexpr int kKeys = D == 256 ? 64 : 128;      // keys of a tile
+    static constexpr int kSoftWarps = 4 * kTilesQ;
+    static constexpr int kThreads = 32 * (kSoftWarps + 2);
+    static constexpr int kQBytes = kTilesQ * kParts * 128 * D * 2;
+    static constexpr int kStageBytes = kKeys * D * 2;      // a tile of K or of V
+    static constexpr int kFixed = 1024 + 512 + kQBytes;
+    static constexpr int kStagesFit = (232448 - kFixed) / kStageBytes;
+    static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
+    static constexpr int kSmem = kFixed + kStages * kStageBytes;
+    static constexpr int kOCol = 2 * kKeys;                // tensor memory: S0 | S1 | O (one per row tile)
+    static_assert(kStages >= 3 && kOCol + kTilesQ * D <= 512, "shared and tensor memory");
+};
+constexpr float kSlack = 6.0f;         // log2 units
+constexpr float kPromptShiftF16 = 8.0f;   // f16 weights are scaled by 2^8: at most 2^14 with the slack, normal down to 2^-22
+
+struct PromptBars {
+    uint64_t full[8], empty[8];
+    uint64_t s_full[2], p_full[2], pv_done[2];
+    uint32_t tmem;
+    int tainted;
+};
+
+// B operand whose rows are the summation index (V as it lies, [key][64 elements] swizzled rows): 8-row groups 1024 bytes
+// apart, runs of 64 elements `run` bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_rows(uint32_t saddr, uint32_t run)
+{
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(run >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__host__ __device__ constexpr uint32_t attend_idesc(bool bf16, int n, bool b_rows)
+{
+    const uint32_t ty = bf16 ? 1u : 0u;
+    return (1u << 4) | (ty << 7) | (ty << 10) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// D += A B with A (16-bit pairs, lane = row) in tensor memory.
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(tmem_d), "r"(tmem_a),
+                 "l"(bdesc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t* v)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+          "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+          "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+        "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+        "r"(v[31])
+        : "memory");
+}
+// The loads issued before are complete; their registers must not be used earlier, which the empty statements pin down.
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[N])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float x, float y)
+{
+    if constexpr (BF16) {
+        __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<uint32_t*>(&h);
+    } else {
+        return h2_as_u32(__floats2half2_rn(x, y));
+    }
+}
+__device__ __forceinline__ float ex2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PromptCfg<T, D>::kThreads, 1)
+attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, KvCacheView c, KvSeqsView s,
+                     RopeView rope, AttendArgs a, int* status)
+{
+    using C = PromptCfg<T, D>;
+    constexpr bool BF = C::kBf16;
+    constexpr int NX = C::kTilesQ, KT = C::kKeys, PRE = 2 / NX, H = D / 64;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* qs = smem;                              // [tile][part][D / 64][128 rows][128 bytes]
+    uint8_t* ring = smem + C::kQBytes;               // [stage][D / 64][KT rows][128 bytes]
+    PromptBars* bar = reinterpret_cast<PromptBars*>(ring + C::kStages * C::kStageBytes);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int group = a.heads / c.heads;
+
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // ---- this CTA's block: blockIdx.y = head, blockIdx.x counts the batch's blocks, each sequence's longest first
+    int seq = 0, blk = (int)blockIdx.x;
+    KvSpan span{};
+    int nb = 0;
+    for (; seq < s.seqs; seq++) {
+        span = kv_span(s, seq);
+        nb = attend_blocks(span, group, C::kRows);
+        if (blk < nb) break;
+        blk -= nb;
+    }
+    if (seq == s.seqs) return;
+    const int head = blockIdx.y;
+    const AttendBlock b = attend_block(c, s, span, group, C::kRows, a.window, nb - 1 - blk);
+    const int t0 = b.lo / KT, tiles = kv_max(1, (b.hi + KT - 1) / KT - t0);
+
+    if (warp == C::kSoftWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < C::kStages; i++) {
+            mbar_init(&bar->full[i], 1);
+            mbar_init(&bar->empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bar->s_full[i], 1);
+            mbar_init(&bar->p_full[i], 4);
+            mbar_init(&bar->pv_done[i], 1);
+        }
+        bar->tainted = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // Q: rotated, scaled to log2 units, in 16-bit parts, K-major with a 128-byte swizzle.  A thread takes one token's 16
+    // elements of two runs of eight (as in the append), its eight angles serving the token's heads.
+    if (warp < C::kSoftWarps) {
+        constexpr int kUnits = D / 16;
+        const int items = (b.j1 - b.j0 + 1) * kUnits;
+        const float scale = a.scale * kLog2e;
+        for (int it = tid; it < items; it += 32 * C::kSoftWarps) {
+            const int u = it % kUnits, j = b.j0 + it / kUnits, pos = span.pos(j);
+            const bool rot = u * 16 < rope.rotary;
+            const int ea = rot && !rope.interleaved ? 8 * u : 16 * u;
+            const int eb = rot && !rope.interleaved ? (rope.rotary >> 1) + 8 * u : 16 * u + 8;
+            float cs[8], sn[8];
+            if (rot) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) rope_cos_sin(rope.turns[8 * u + i], pos, &cs[i], &sn[i]);
+            }
+            const int g0 = kv_max(0, b.r0 - j * group), g1 = kv_min(group, b.r0 + b.rows - j * group);
+            for (int g = g0; g < g1; g++) {
+                const float* q = a.q + (size_t)(span.first + j) * a.ldq + (size_t)(head * group + g) * D;
+                float x[16];
+                *reinterpret_cast<float4*>(x) = ld_act(reinterpret_cast<const float4*>(q + ea));
+                *reinterpret_cast<float4*>(x + 4) = ld_act(reinterpret_cast<const float4*>(q + ea + 4));
+                *reinterpret_cast<float4*>(x + 8) = ld_act(reinterpret_cast<const float4*>(q + eb));
+                *reinterpret_cast<float4*>(x + 12) = ld_act(reinterpret_cast<const float4*>(q + eb + 4));
+                if (rot) rope_rotate16(x, cs, sn, rope.interleaved);
+                const int row = j * group + g - b.r0, tile = row >> 7, rr = row & 127;
+                uint8_t* base = qs + tile * (C::kParts * 128 * D * 2) + rr * 128;
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[i] *= scale;
+#pragma unroll
+                for (int part = 0; part < C::kParts; part++) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        w[i] = pack2<BF>(x[2 * i], x[2 * i + 1]);
+                        if (BF) {
+                            x[2 * i] -= __uint_as_float(w[i] << 16);
+                            x[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+                        }
+                    }
+                    uint8_t* p = base + part * (128 * D * 2);
+                    const int ca = ea >> 3, cb = eb >> 3;
+                    *reinterpret_cast<uint4*>(p + (ca >> 3) * (128 * 128) + (((ca & 7) ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(p + (cb >> 3) * (128 * 128) + (((cb & 7) ^ (rr & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+            }
+        }
+        // rows the block does not have
+        for (int i = tid + b.rows * (D / 8); i < C::kRows * (D / 8); i += 32 * C::kSoftWarps) {
+            const int row = i / (D / 8), ch = i % (D / 8);
+#pragma unroll
+            for (int part = 0; part < C::kParts; part++)
+                *reinterpret_cast<uint4*>(qs + (row >> 7) * (C::kParts * 128 * D * 2) + part * (128 * D * 2) + (ch >> 3) * (128 * 128) + (row & 127) * 128 +
+                                          ((ch & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar->tmem;
+    bool dead = false;                        // a wait ran out: wait for nothing more, finish the launch
+    auto wait = [&](uint64_t* which, uint32_t parity, int code) {
+        if (dead || mbar_wait(which, parity)) return;
+        dead = true;
+        if (status) atomicExch(status, code);
+    };
+    // keys every row of the block sees: tiles inside need no mask
+    const int lo_all = kv_seen_lo(span.pos(b.j1), a.window), hi_all = kv_seen_hi(c, s, span.pos(b.j0));
+
+    if (warp == C::kSoftWarps + 1) {
+        // ---- loader: K0 (.. K1), then V_j and K_{j + PRE} in turn, the order in which the products first use them
+        const int box = kv_min(kAttendTile, 1 << c.page_shift), pp = KT / box, copies = pp * H;
+        const int piece = lane % pp, half = (lane / pp) % H;
+        int n = 0;
+        auto load = [&](const CUtensorMap* map, int j) {
+            const int st = n % C::kStages, pos = (t0 + j) * KT + piece * box;
+            const int page = kv_page(c, s, seq, pos >> c.page_shift);
+            if (n >= C::kStages) wait(&bar->empty[st], ((n / C::kStages) & 1) ^ 1, 50);
+            if (lane == 0) mbar_expect_tx(&bar->full[st], C::kStageBytes);
+            __syncwarp();
+            if (lane < copies)
+                tma_load_4d(ring + st * C::kStageBytes + half * (KT * 128) + piece * box * 128, map, half * 64, pos & ((1 << c.page_shift) - 1), head,
+                            page >= 0 ? page : max(1, c.n_pages), &bar->full[st]);
+            n++;
+        };
+        for (int j = 0; j < kv_min(PRE, tiles); j++) load(&kmap, j);
+        for (int j = 0; j < tiles; j++) {
+            const int mine = n;
+            load(&vmap, j);
+            if (j + PRE < tiles) load(&kmap, j + PRE);
+            // A tile that some rows see and others do not: an infinity or NaN among its values would reach all of them through
+            // the product.  Such a block is done again key by key (below); the tile cannot be refilled before this warp says so.
+            const int k0 = (t0 + j) * KT;
+            if (b.j0 != b.j1 && (k0 < lo_all || k0 + KT > hi_all)) {
+                const int st = mine % C::kStages;
+                wait(&bar->full[st], (mine / C::kStages) & 1, 51);
+                bool odd = false;
+                for (int i = lane; i < KT * (D / 8); i += 32) {
+                    const int row = (i >> 3) % KT, hf = i / (8 * KT);
+                    const uint4 w = *reinterpret_cast<const uint4*>(ring + st * C::kStageBytes + hf * (KT * 128) + row * 128 + ((i & 7) << 4));
+                    constexpr uint32_t e = BF ? 0x7f80u : 0x7c00u;
+                    auto bad = [&](uint32_t v) { return (v & e) == e || (v & (e << 16)) == (e << 16); };
+                    if (k0 + row >= b.lo && k0 + row < b.hi) odd |= bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
+                }
+                if (odd) bar->tainted = 1;
+                __syncwarp();
+            }
+        }
+    } else if (warp == C::kSoftWarps) {
+        // ---- products.  Unit u = (key tile u / NX, row tile u % NX), S buffer u & 1.
+        const uint32_t qbase = smem_u32(qs), rbase = smem_u32(ring);
+        const int units = tiles * NX;
+        constexpr uint32_t id_s = attend_idesc(BF, KT, false), id_o = attend_idesc(BF, D, true);
+        int n = 0;                            // ring position
+        int k_st = 0, v_st = 0;
+        auto issue_s = [&](int u) {
+            const int x = u % NX;
+            if (x == 0) {
+                k_st = n % C::kStages;
+                wait(&bar->full[k_st], (n / C::kStages) & 1, 52);
+                n++;
+            }
+            tc_fence_after();
+            if (lane == 0 && !dead) {
+                const uint32_t kb = umma_desc_lo(rbase + k_st * C::kStageBytes);
+#pragma unroll
+                for (int part = 0; part < C::kParts; part++) {
+                    const uint32_t qb = umma_desc_lo(qbase + (x * C::kParts + part) * (128 * D * 2));
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ks++)
+                        umma_f16_lo(tmem + (u & 1) * KT, qb + (ks >> 2) * (128 * 128 / 16) + (ks & 3) * 2, kb + (ks >> 2) * (KT * 128 / 16) + (ks & 3) * 2,
+                                    id_s, part > 0 || ks > 0);
+                }
+                if (x == NX - 1) umma_commit(&bar->empty[k_st]);
+                umma_commit(&bar->s_full[u & 1]);
+            }
+            __syncwarp();
+        };
+        for (int u = 0; u < kv_min(2, units); u++) issue_s(u);
+        for (int u = 0; u < units; u++) {
+            const int x = u % NX, j = u / NX;
+            if (x == 0) {
+                v_st = n % C::kStages;
+                wait(&bar->full[v_st], (n / C::kStages) & 1, 53);
+                n++;
+                // keys outside what any row sees have weight 0; their values must not be infinities or NaN
+                const int k0 = (t0 + j) * KT, z0 = kv_max(0, b.lo - k0), z1 = kv_min(KT, b.hi - k0);
+                if (z0 > 0 || z1 < KT) {
+                    for (int i = lane; i < KT * (D / 8); i += 32) {
+                        const int row = (i >> 3) % KT, hf = i / (8 * KT);
+                        if (row < z0 || row >= z1)
+                            *reinterpret_cast<uint4*>(ring + v_st * C::kStageBytes + hf * (KT * 128) + row * 128 + ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+            }
+            wait(&bar->p_full[u & 1], (u >> 1) & 1, 54);
+            tc_fence_after();
+            if (lane == 0 && !dead) {
+#pragma unroll
+                for (int kk = 0; kk < KT / 16; kk++)
+                    umma_ts(tmem + C::kOCol + x * D, tmem + (u & 1) * KT + kk * 8, umma_desc_rows(rbase + v_st * C::kStageBytes + kk * 2048, KT * 128), id_o,
+                            j > 0 || kk > 0);
+                if (x == NX - 1) umma_commit(&bar->empty[v_st]);
+                umma_commit(&bar->pv_done[x]);
+            }
+            __syncwarp();
+            if (u + 2 < units) issue_s(u + 2);
+        }
+    } else {
+        // ---- softmax: thread = row
+        const int x = warp >> 2, row = x * 128 + (warp & 3) * 32 + lane, r = b.r0 + row;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int j_tok = r / group;
+        const bool have = row < b.rows;
+        const int lo_r = have ? kv_seen_lo(span.pos(j_tok), a.window) : 0, hi_r = have ? kv_seen_hi(c, s, span.pos(j_tok)) : 0;
+        const int run = kv_min(KT == 128 ? 7 : 6, c.page_shift), pages = KT >> run;
+        constexpr float kShift = BF ? 0.0f : kPromptShiftF16;
+        float m = -INFINITY, l = 0.0f;      // weights are 2^(s - m)
+        for (int j = 0; j < tiles; j++) {
+            const int u = j * NX + x, sb = u & 1, k0 = (t0 + j) * KT;
+            const unsigned valid = __ballot_sync(0xffffffffu, lane < pages && kv_page(c, s, seq, (k0 + (lane << run)) >> c.page_shift) >= 0);
+            wait(&bar->s_full[sb], (u >> 1) & 1, 55);
+            tc_fence_after();
+            uint32_t w[KT];
+#pragma unroll
+            for (int i = 0; i < KT / 32; i++) tmem_ld32_nowait(tmem + lanes + sb * KT + 32 * i, w + 32 * i);
+            tmem_wait_ld(w);
+            if (k0 < lo_all || k0 + KT > hi_all || valid != (1u << pages) - 1u) {
+#pragma unroll
+                for (int i = 0; i < KT; i++) {
+                    const int key = k0 + i;
+                    const bool page = (valid >> (i >> run)) & 1u;
+                    if (!(key >= lo_r && key < hi_r && page)) w[i] = 0xff800000u;   // -inf
+                }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < KT; i += 2)
+                asm("max.f32 %0, %0, %1, %2;" : "+f"(mx) : "f"(__uint_as_float(w[i])), "f"(__uint_as_float(w[i + 1])));
+            mx -= kShift;
+            const bool move = mx > m + kSlack || (m == -INFINITY && mx > m);
+            if (__any_sync(0xffffffffu, move)) {
+                const float mn = move ? mx : m, fix = move ? ex2_approx(m - mn) : 1.0f;
+                m = mn;
+                l *= fix;
+                if (j > 0) {
+                    // O of the units before must be complete
+                    wait(&bar->pv_done[x], (j - 1) & 1, 56);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int i = 0; i < D / 32; i++) {
+                        uint32_t v[32];
+                        tmem_ld32_nowait(tmem + lanes + C::kOCol + x * D + 32 * i, v);
+                        tmem_wait_ld(v);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * fix);
+                        tmem_st32(tmem + lanes + C::kOCol + x * D + 32 * i, v);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KT / 2; i++) {
+                const float p0 = ex2_approx(__uint_as_float(w[2 * i]) - base), p1 = ex2_approx(__uint_as_float(w[2 * i + 1]) - base);
+                sum0 += p0;
+                sum1 += p1;
+                w[i] = pack2<BF>(p0, p1);
+            }
+            l += sum0 + sum1;
+#pragma unroll
+            for (int i = 0; i < KT / 64; i++) tmem_st32(tmem + lanes + sb * KT + 32 * i, w + 32 * i);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->p_full[sb]);
+        }
+        wait(&bar->pv_done[x], (tiles - 1) & 1, 57);
+        tc_fence_after();
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + j_tok) * a.ldo + (size_t)(head * group + r % group) * D;
+#pragma unroll 1
+        for (int i = 0; i < D / 32; i++) {
+            uint32_t v[32];
+            tmem_ld32_nowait(tmem + lanes + C::kOCol + x * D + 32 * i, v);
+            tmem_wait_ld(v);
+            if (have) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        y[k] = pack2<true>(__uint_as_float(v[8 * e + 2 * k]) * inv, __uint_as_float(v[8 * e + 2 * k + 1]) * inv);
+                    *reinterpret_cast<uint4*>(out + 32 * i + 8 * e) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == C::kSoftWarps)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    if (bar->tainted) {
+        // the rows one by one, key by key (what was stored above is overwritten)
+        float* q = reinterpret_cast<float*>(qs) + warp * D;
+        for (int row = warp; row < b.rows; row += C::kThreads / 32) {
+            const int j = (b.r0 + row) / group, h = head * group + (b.r0 + row) % group, pos = span.pos(j);
+            const float* src = a.q + (size_t)(span.first + j) * a.ldq + (size_t)h * D;
+            __syncwarp();
+            for (int e = lane; e < D; e += 32) q[e] = rope_element(rope, src, e, pos) * (a.scale * kLog2e);
+            __syncwarp();
+            float m, l, acc[D / 32];
+            attend_row_plain<T, D>(c, s, seq, head, q, kv_seen_lo(pos, a.window), kv_seen_hi(c, s, pos), lane, &m, &l, acc);
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + j) * a.ldo + (size_t)h * D;
+#pragma unroll
+            for (int e = 0; e < D / 32; e++) out[lane + 32 * e] = __float2bfloat16_rn(acc[e] * inv);
+        }
+    }
+}
+
+namespace {
+template <typename T, int D>
+int32_t launch_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a, const GemvTuning& tune)
+{
+    using C = PromptCfg<T, D>;
+    static bool attr_done[64] = {};
+    int dev = 0;
+    FERRIC_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 64 || !attr_done[dev]) {
+        FERRIC_CUDA_TRY(cudaFuncSetAttribute(attend_prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        if (dev < 64) attr_done[dev] = true;
+    }
+    CUtensorMap kmap, vmap;
+    int32_t rc;
+    if ((rc = encode_cache(&kmap, c, c.k, a.q)) != kOk || (rc = encode_cache(&vmap, c, c.v, a.q)) != kOk) return rc;
+    // the batch's spans are on the device: as many blocks as any could make, those behind the last return at once
+    const long long blocks = ((long long)s.tokens * (a.heads / c.heads)) / C::kRows + s.seqs;
+    FERRIC_CUDA_TRY(launch_kernel(attend_prompt_kernel<T, D>, dim3((unsigned)blocks, (unsigned)c.heads), dim3(C::kThreads), C::kSmem, st, tune.pdl, kmap, vmap,
+                                  c, s, r, a, gemm_status_word()));
+    return kOk;
+}
+}  // namespace
+
+// Prompts pay for tiles of 256 query rows (one sequence's tokens x query heads per key-value head) and whole CTAs per block;
+// below that, and where a result is wanted in f32, the split kernel runs.
+bool attend_prompt_eligible(const KvCacheView& c, const KvSeqsView& s, const AttendArgs& a)
+{
+    if (!a.out_bf16) return false;
+    const long long rows = (long long)s.tokens / s.seqs * (a.heads / c.heads);
+    return rows >= 128;
+}
+int32_t launch_attend_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a, const GemvTuning& tune)
+{
+    switch (c.dim) {
+    case 64: return c.bf16 ? launch_prompt<__nv_bfloat16, 64>(st, c, s, r, a, tune) : launch_prompt<__half, 64>(st, c, s, r, a, tune);
+    case 128: return c.bf16 ? launch_prompt<__nv_bfloat16, 128>(st, c, s, r, a, tune) : launch_prompt<__half, 128>(st, c, s, r, a, tune);
+    default: return c.bf16 ? launch_prompt<__nv_bfloat16, 256>(st, c, s, r, a, tune) : launch_prompt<__half, 256>(st, c, s, r, a, tune);
+    }
+}
+
+}  // namespace ferric

@@ -53,15 +53,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvCacheView c, KvSeqsVie
         *reinterpret_cast<float4*>(a + 12) = ld_act(reinterpret_cast<const float4*>(kr + eb + 4));
 #pragma unroll
         for (int e = 0; e < 4; e++) *reinterpret_cast<float4*>(w + 4 * e) = ld_act(reinterpret_cast<const float4*>(vr + 4 * e));
-        if (rot) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int i0 = r.interleaved ? 2 * e : e, i1 = r.interleaved ? 2 * e + 1 : e + 8;
-                const float x = a[i0], y = a[i1];
-                a[i0] = fmaf(-y, sn[e], x * cs[e]);
-                a[i1] = fmaf(y, cs[e], x * sn[e]);
-            }
-        }
+        if (rot) rope_rotate16(a, cs, sn, r.interleaved);
         T ko[16], vo[16];
 #pragma unroll
         for (int e = 0; e < 16; e++) {

@@ -32,6 +32,26 @@ __device__ __forceinline__ float rope_element(const RopeView& r, const float* x,
     return e < half ? fmaf(-x[e + half], s, x[e] * c) : fmaf(x[e - half], s, x[e] * c);
 }
 
+// Eight pairs at once: the two runs of eight elements x[0..8) and x[8..16) (pairs across the runs), or sixteen adjacent ones.
+__device__ __forceinline__ void rope_rotate16(float (&x)[16], const float (&cs)[8], const float (&sn)[8], int interleaved)
+{
+    if (interleaved) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float a = x[2 * e], b = x[2 * e + 1];
+            x[2 * e] = fmaf(-b, sn[e], a * cs[e]);
+            x[2 * e + 1] = fmaf(b, cs[e], a * sn[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float a = x[e], b = x[e + 8];
+            x[e] = fmaf(-b, sn[e], a * cs[e]);
+            x[e + 8] = fmaf(b, cs[e], a * sn[e]);
+        }
+    }
+}
+
 __device__ __forceinline__ float kv_to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float kv_to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void kv_from_float(float v, __half* o) { *o = __float2half_rn(v); }
