@@ -2,10 +2,11 @@
 
 One layer is the matmul sequence of ``Qwen35::forward_cached`` (crates/ferric-llama/src/qwen35.rs:953-1014,
 ffn :834-840): rmsnorm -> fused q|k|v projection -> [mixer] -> o projection -> add_rmsnorm ->
-fused gate|up + SwiGLU -> down projection -> add.  Attention / GDN and the KV cache are outside this
-backend's scope, so the mixer is a pass-through: the q slice of the qkv output feeds the o
-projection.  Everything else (shapes, formats, fusion of q|k|v and gate|up into one matrix as
-``qm_cat`` does, :380-402) is as the model runs it.
+fused gate|up + SwiGLU -> down projection -> add.  The mixer is attention over a paged key-value cache where the
+stack is given one (``Attention``, the attn layers of :665-724); by default it is a pass-through, the q slice of the qkv
+output feeding the o projection, which is what the products are measured with.  GDN layers are outside this backend's
+scope.  Everything else (shapes, formats, fusion of q|k|v and gate|up into one matrix as ``qm_cat`` does, :380-402) is as
+the model runs it.
 
 Tensor parallelism (one process per GPU): q|k|v and gate|up are split by output rows, o and down by
 input columns on 256-weight super-block boundaries, and the f32 [B, hidden] partial sums of o and
@@ -20,7 +21,7 @@ from typing import Callable, List, Optional
 import torch
 
 from . import synth
-from .ops import Context, QMatrix, TPGroup, GGML_Q4_K, GGML_Q6_K
+from .ops import Context, KVCache, KVSeqs, QMatrix, Rope, TPGroup, GGML_Q4_K, GGML_Q6_K
 
 
 def split_blocks(total_blocks: int, world: int) -> List[int]:
@@ -69,6 +70,22 @@ class TPPlan:
 AllReduce = Callable[[torch.Tensor], None]
 
 
+@dataclass(frozen=True)
+class Attention:
+    """The stack's attention: heads of ``head_dim`` (as many as the q and k / v widths hold), ``max_len`` positions per
+    sequence in pages of ``page_size``, keys and values in ``dtype``, RoPE over the first ``rotary`` elements (None: all; 0:
+    none)."""
+    head_dim: int = 128
+    max_len: int = 4096
+    page_size: int = 64
+    dtype: torch.dtype = torch.bfloat16
+    rope_base: float = 1.0e6
+    rotary: Optional[int] = None
+    interleaved: bool = False
+    window: int = 0
+    scale: Optional[float] = None
+
+
 class Layer:
     def __init__(self, wqkv: QMatrix, wo: QMatrix, wgu: QMatrix, wdown: QMatrix):
         self.wqkv, self.wo, self.wgu, self.wdown = wqkv, wo, wgu, wdown
@@ -83,8 +100,11 @@ class DecodeStack:
 
     def __init__(self, ctx: Context, plan: TPPlan, n_layers: int = 64, batch: int = 1, eps: float = 1e-6,
                  all_reduce: Optional[AllReduce] = None, group: Optional[TPGroup] = None, push: bool = True,
-                 chain: Optional[bool] = None):
-        """`all_reduce`: a callable summing a tensor over ranks in place (e.g. NCCL through torch.distributed).
+                 chain: Optional[bool] = None, attention: Optional[Attention] = None):
+        """`attention`: attend over a key-value cache (one per layer, one sequence per token of the batch) between q|k|v and o;
+        every step appends one token per sequence.  One rank, unchained: the attention reads the finished q|k|v rows, so
+        there is nothing for q|k|v's launch to prepare for o.
+        `all_reduce`: a callable summing a tensor over ranks in place (e.g. NCCL through torch.distributed).
         `group`: a connected TPGroup -- then the exchange is done by this library's own kernels instead; with
         `push` the o / down products store their partial sums straight into every rank's memory, otherwise each
         rank signals its buffer and the consumers read the peers' buffers.
@@ -96,6 +116,12 @@ class DecodeStack:
         (3.77 against 3.46 ms per step on 2 GPUs)."""
         self.ctx, self.plan, self.n_layers, self.batch, self.eps = ctx, plan, n_layers, batch, eps
         can_chain = batch <= 4 and (plan.world == 1 or (group is not None and push))
+        if attention is not None:
+            if plan.world > 1:
+                raise ValueError("attention needs whole key-value groups: one rank")
+            if chain:
+                raise ValueError("a chained step has no place for attention between q|k|v and o")
+            chain = False
         self.chain = (can_chain and batch <= 2 and plan.world == 1) if chain is None else (chain and can_chain)
         self.all_reduce = all_reduce if (plan.world > 1 and group is None) else None
         self.group = group if plan.world > 1 else None
@@ -117,6 +143,51 @@ class DecodeStack:
             self.d = torch.empty((B, p.hidden), **f32)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.launches_per_step = 0
+        self.attention = attention
+        if attention is not None:
+            self._init_attention(attention, dev)
+
+    def _init_attention(self, a: Attention, dev: torch.device) -> None:
+        p, B, d = self.plan, self.batch, a.head_dim
+        if p.q_rows % d or p.kv_rows % d or (p.q_rows // d) % (p.kv_rows // d):
+            raise ValueError(f"q width {p.q_rows} and k / v width {p.kv_rows} are not heads of {d} in whole groups")
+        pages = -(-a.max_len // a.page_size)
+        table = torch.arange(B * pages, dtype=torch.int32, device=dev).reshape(B, pages)
+        self.seqs = KVSeqs(table, torch.zeros(B, dtype=torch.int32, device=dev))
+        rotary = d if a.rotary is None else a.rotary
+        self.rope = Rope(self.ctx, rotary, a.rope_base, a.interleaved) if rotary else None
+        self.caches = [KVCache.empty(self.ctx, B * pages, a.page_size, p.kv_rows // d, d, a.dtype) for _ in range(self.n_layers)]
+        self.att = torch.empty((B, p.q_rows), dtype=torch.float32, device=dev)
+        self.longest = 0        # tokens in the longest sequence, kept on the host beside the device's lengths
+
+    def set_lengths(self, lens) -> None:
+        """The number of tokens each sequence's cache holds (what a prompt left there, or 0 to start over)."""
+        lens = [int(n) for n in lens]
+        if len(lens) != self.batch or min(lens) < 0 or max(lens) > self.attention.max_len:
+            raise ValueError(f"{self.batch} lengths within [0, {self.attention.max_len}], not {lens}")
+        self.seqs.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        self.longest = max(lens)
+
+    def _mix(self, i: int) -> torch.Tensor:
+        """What feeds layer i's o projection: the attention's result, or the q slice as it is."""
+        p, a = self.plan, self.attention
+        q = self.qkv[:, :p.q_rows]
+        if a is None:
+            return q
+        c = self.caches[i]
+        c.append(self.seqs, self.qkv[:, p.q_rows:p.q_rows + p.kv_rows], self.qkv[:, p.q_rows + p.kv_rows:], rope=self.rope)
+        return c.attend(self.seqs, q, rope=self.rope, scale=a.scale, window=a.window, out=self.att)
+
+    def _begin_token(self) -> None:
+        """One more token per sequence: on the device (captured with the step), checked on the host."""
+        if self.attention is not None:
+            self._room()
+            self.seqs.lens.add_(1)
+
+    def _room(self) -> None:
+        if self.longest >= self.attention.max_len:
+            raise RuntimeError(f"the cache is full: {self.longest} tokens, max_len {self.attention.max_len}")
+        self.longest += 1
 
     # -- weights ---------------------------------------------------------------------------
     def add_layer(self, wqkv: QMatrix, wo: QMatrix, wgu: QMatrix, wdown: QMatrix) -> None:
@@ -166,6 +237,7 @@ class DecodeStack:
         c, p = self.ctx, self.plan
         before = c.launches()
         n = len(self.layers)
+        self._begin_token()
         if self.batch > 8:
             return self._step_wide(before)
         if self.chain:
@@ -182,7 +254,7 @@ class DecodeStack:
                 G.signal(0)
                 G.add_rmsnorm_prepare(0, L.wgu, self.h, None, self.eps, sum_out=self.h)
             else:
-                L.wo.matmul(self.qkv[:, :p.q_rows], out=self.o)
+                L.wo.matmul(self._mix(i), out=self.o)
                 if self.all_reduce:
                     self.all_reduce(self.o)
                 L.wgu.add_rmsnorm_prepare(self.h, self.o, None, self.eps, sum_out=self.h)
@@ -240,7 +312,7 @@ class DecodeStack:
                 self.group.matmul_scatter(0, L.wo, self.qkv[:, :p.q_rows])
                 self.group.allreduce_add_rmsnorm(0, self.o, self.h, None, self.eps, sum_out=self.h, norm_out=self.xn, steps=6)
             else:
-                L.wo.matmul(self.qkv[:, :p.q_rows], out=self.o)
+                L.wo.matmul(self._mix(i), out=self.o)
                 if self.all_reduce:
                     self.all_reduce(self.o)
                 c.add_rmsnorm(self.h, self.o, None, self.eps, sum_out=self.h, norm_out=self.xn)
@@ -258,7 +330,12 @@ class DecodeStack:
         return self.h
 
     def capture(self, warmup: int = 2) -> None:
-        """Record one step into a CUDA graph (launch-bound loop: ~10 kernels per layer)."""
+        """Record one step into a CUDA graph (launch-bound loop: ~10 kernels per layer).  The warm-up steps leave the caches
+        alone: with lengths below 0 their tokens have no position."""
+        if self.attention is not None:
+            lens, longest = self.seqs.lens.clone(), self.longest
+            self.longest = -warmup - 1
+            self.seqs.lens.fill_(self.longest)
         side = torch.cuda.Stream(device=self.ctx.device)
         side.wait_stream(torch.cuda.current_stream(self.ctx.device))
         with torch.cuda.stream(side):
@@ -272,10 +349,15 @@ class DecodeStack:
             self.ctx.use_torch_stream()
             self.step()
         self.ctx.use_torch_stream()
+        if self.attention is not None:
+            self.seqs.lens.copy_(lens)
+            self.longest = longest
         self.graph = g
 
     def run(self) -> torch.Tensor:
         if self.graph is not None:
+            if self.attention is not None:
+                self._room()
             self.graph.replay()
             return self.h
         return self.step()

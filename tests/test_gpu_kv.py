@@ -474,6 +474,104 @@ def test_a_cache_past_32_bit_offsets(F, ctx):
         assert ((y - want).abs() <= bound).all()
 
 
+# ---- the decoder stack with attention -----------------------------------------------------------------------
+def stack_of(F, ctx, batch, **kw):
+    from ferric_b200.stack import Attention, DecodeStack, TPPlan
+    plan = TPPlan.make(1, 0, hidden=512, n_ff=512, q_out=512, kv_out=256)
+    st = DecodeStack(ctx, plan, n_layers=2, batch=batch, attention=Attention(max_len=40, page_size=16, dtype=HF, scale=2e-3, **kw))
+    st.build_synthetic(seed=3)
+    return st
+
+
+@pytest.mark.parametrize("batch", [3, 12])
+def test_stack_with_attention(F, ctx, batch):
+    """Append + attend between q|k|v and o, step after step, then captured.  The first layer's cache against 64 bits (its input
+    is the test's own); everything behind it bit for bit against the operators called one by one -- the attention itself is
+    held to 64 bits above, and behind a softmax over scores of hundreds a difference of 1e-5 in a score is one of 1e-5 in a
+    weight, which the next layers multiply: no bar on the products bounds what it becomes."""
+    st = stack_of(F, ctx, batch)
+    wqkv0 = st.layers[0].wqkv.dequant().double().cpu()
+    g = torch.Generator().manual_seed(9)
+    rope = dict(rotary=128, base=1e6)
+    mine = [F.KVCache.empty(ctx, c.k.shape[0], 16, 2, 128, HF) for c in st.caches]
+    for c, d in zip(st.caches, mine):
+        for t in (c.k, c.v, d.k, d.v):
+            t.zero_()
+    lens = [0] * batch
+    for step in range(6):
+        if step == 3:                                  # some sequences start over
+            lens = [0 if i % 2 else n for i, n in enumerate(lens)]
+            st.set_lengths(lens)
+            before = [(c.k.clone(), c.v.clone()) for c in st.caches]
+            st.capture()                               # the rest replays
+            assert st.seqs.lens.tolist() == lens
+            for c, (k, v) in zip(st.caches, before):   # its warm-up steps appended nothing
+                assert torch.equal(c.k, k) and torch.equal(c.v, v)
+        x = torch.randn((batch, 512), generator=g)
+        st.h.copy_(x)
+        st.run()
+        lens = [n + 1 for n in lens]
+        assert st.seqs.lens.tolist() == lens
+        seqs = F.KVSeqs(st.seqs.page_table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+        h = x.cuda()
+        for i, L in enumerate(st.layers):
+            if batch > 8:
+                if i == 0:
+                    _, xn = ctx.add_rmsnorm(h, None, None, st.eps)
+                qkv = L.wqkv.matmul(xn)
+            else:
+                if i == 0:
+                    m = L.wqkv.add_rmsnorm_prepare(h, None, None, st.eps)
+                qkv = L.wqkv.matmul_prepared(m)
+            mine[i].append(seqs, qkv[:, 512:768], qkv[:, 768:], rope=st.rope)
+            o = L.wo.matmul(mine[i].attend(seqs, qkv[:, :512], rope=st.rope, scale=2e-3))
+            nxt = st.layers[(i + 1) % 2].wqkv
+            if batch > 8:
+                h, xn = ctx.add_rmsnorm(h, o, None, st.eps)
+                h, xn = ctx.add_rmsnorm(h, L.wdown.matmul(L.wgu.try_matmul_swiglu(xn)), None, st.eps)
+            else:
+                s2, xn = torch.empty_like(h), torch.empty_like(h)
+                m = L.wgu.add_rmsnorm_prepare(h, o, None, st.eps, sum_out=s2)
+                d = L.wdown.matmul(L.wgu.matmul_prepared(m, swiglu=True))
+                h = torch.empty_like(h)
+                m = nxt.add_rmsnorm_prepare(s2, d, None, st.eps, sum_out=h, norm_out=xn)
+            assert torch.equal(mine[i].k, st.caches[i].k) and torch.equal(mine[i].v, st.caches[i].v)
+        assert torch.equal(st.h, h) and torch.equal(st.xn, xn)
+        # a rotated element is a cos - b sin, so the products' bar (1e-4 + 1e-3 |.|) counts for both of its pair
+        hx = x.double()
+        qkv = (hx / (hx.pow(2).mean(-1, keepdim=True) + st.eps).sqrt()) @ wqkv0.T
+        c = st.caches[0]
+        kx, vx, mag, written = R.append(c.k, c.v, st.seqs.page_table.cpu(), lens, None, qkv[:, 512:768], qkv[:, 768:], rope)
+        mag = mag * 2.0 ** 21
+        assert ((c.k.double().cpu() - kx)[written].abs() <= 2e-4 + 1.001e-3 * mag[written] + 2.0 ** -11 * kx[written].abs()).all()
+        assert ((c.v.double().cpu() - vx)[written].abs() <= 1e-4 + (1e-3 + 2.0 ** -11) * vx[written].abs()).all()
+    st.close()
+
+
+def test_stack_refuses_what_it_cannot_hold(F, ctx):
+    from ferric_b200.stack import Attention, DecodeStack, TPPlan
+    st = stack_of(F, ctx, 2)
+    st.set_lengths([39, 3])
+    st.h.normal_()
+    st.step()
+    with pytest.raises(RuntimeError):
+        st.step()
+    assert st.seqs.lens.tolist() == [40, 4]
+    with pytest.raises(ValueError):
+        st.set_lengths([41, 0])
+    with pytest.raises(ValueError):
+        st.set_lengths([1])
+    plan = TPPlan.make(1, 0, hidden=512, n_ff=512, q_out=512, kv_out=256)
+    with pytest.raises(ValueError):
+        DecodeStack(ctx, plan, n_layers=1, chain=True, attention=Attention())
+    with pytest.raises(ValueError):
+        DecodeStack(ctx, plan, n_layers=1, attention=Attention(head_dim=192))
+    with pytest.raises(ValueError):
+        DecodeStack(ctx, TPPlan.make(2, 0, hidden=512, n_ff=512, q_out=512, kv_out=256), n_layers=1, all_reduce=lambda t: None,
+                    attention=Attention())
+    st.close()
+
+
 # ---- refusals -----------------------------------------------------------------------------------------------
 def test_refusals(F, ctx):
     b = Batch(F, ctx, lens=[20, 30])
