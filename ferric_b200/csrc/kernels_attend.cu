@@ -39,10 +39,14 @@ struct SplitCfg {
     static constexpr int kStageBytes = 2 * kAttendTile * D * 2;
     static constexpr bool kQSmem = D == 256;             // 96 registers of q and 128 of output do not fit one thread
     static constexpr int kQBytes = kQSmem ? WM * (D / 16) * 32 * (kBf16 ? 24 : 16) : 0;
-    static constexpr int kPitch = D + 8;                 // a row of results: D sums, m, l
-    static constexpr int kBufRows = kRows + kWarps > 16 ? kRows + kWarps : 16;
-    static constexpr int kBufFloats = kBufRows * kPitch;   // q rows; halves of the warps' results; results; pieces' (m, l)
-    static constexpr int kFixed = 1024 + kQBytes + kBufFloats * 4 + 512;
+    static constexpr int kPitch = D + 8;                 // floats of a row of q, or of results: D sums, m, l
+    // warps that hand their results over in one round of the merge
+    static constexpr int kMerge = kWN == 1 ? 0 : (D == 256 && WM == 1) ? 1 : kWarps / 2;
+    static constexpr int kSlot = 8 * D + 32;
+    static constexpr int kBufFloats = kMerge * kSlot > kRows * kPitch ? kMerge * kSlot : kRows * kPitch;   // merge; results; pieces' (m, l)
+    // the widest tiles at head_dim 256 keep q and the results in one place: the next block's q comes when this one is done
+    static constexpr bool kOneBuf = D == 256 && WM == 4;
+    static constexpr int kFixed = 1024 + kQBytes + (kOneBuf ? 0 : kRows * kPitch * 4) + kBufFloats * 4 + 512;
     // Two CTAs per SM where registers and shared memory allow: one CTA's set-up and join hide under the other's stream.
     static constexpr int kMinCtas = (D == 256 || WM == 8) ? 1 : 2;
     static constexpr int kSmemMax = kMinCtas == 2 ? 113 * 1024 : 227 * 1024;
@@ -59,11 +63,12 @@ struct SplitWork {
     unsigned* tickets;   // [CTA], zero between launches
     int* status;
     int min_tiles;       // tiles per CTA at least, while there are few
+    unsigned long long group_recip;   // ceil(2^32 / group)
 };
 struct SplitBars {
-    uint64_t full[8], empty[8];
+    uint64_t full[8], empty[8], q_full, q_empty;
     unsigned valid[8];           // per stage: which of the tile's pages exist
-    unsigned long long total;
+    long long warp_sum[16];
     long long item_start;
     int seq, tainted, last;
 };
@@ -135,7 +140,8 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* qfrag = ring + C::kStages * C::kStageBytes;
-    float* buf = reinterpret_cast<float*>(qfrag + C::kQBytes);
+    float* qrow = reinterpret_cast<float*>(qfrag + C::kQBytes);   // the block's q rows, rotated in place
+    float* buf = C::kOneBuf ? qrow : qrow + C::kRows * C::kPitch;
     SplitBars* bar = reinterpret_cast<SplitBars*>(buf + C::kBufFloats);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.heads / c.heads;
@@ -145,10 +151,18 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             mbar_init(&bar->full[i], 1);
             mbar_init(&bar->empty[i], C::kWarps);
         }
+        mbar_init(&bar->q_full, 1);
+        mbar_init(&bar->q_empty, C::kWarps);
         bar->tainted = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_launch_dependents();
+    // this thread's pair of elements of a q row and its frequency (immutable: read before the wait)
+    constexpr int kPairs = D / 2, kCons = 32 * C::kWarps;
+    const int pair = tid % kPairs;
+    const bool rot = 2 * pair < rope.rotary;
+    const int e0 = rot && !rope.interleaved ? pair : 2 * pair, e1 = rot && !rope.interleaved ? pair + (rope.rotary >> 1) : 2 * pair + 1;
+    const double turns = rot ? rope.turns[pair] : 0.0;
     pdl_wait();
 
     // ---- this CTA's run of tiles: the batch's total, then the sequence in which the run starts
@@ -156,28 +170,32 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     auto seq_tiles = [&](int i) -> long long {
         return i < s.seqs ? attend_seq_tiles(c, s, kv_span(s, i), group, RB, a.window) * c.heads : 0;
     };
-    auto warp_incl = [&](long long v) {
+    // inclusive sum over the block's threads; `all` is the sum over all of them
+    auto block_incl = [&](long long v, long long* all) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
-        return v;
+        if (lane == 31) bar->warp_sum[warp] = v;
+        __syncthreads();
+        long long before = 0, sum = 0;
+#pragma unroll
+        for (int w = 0; w < C::kWarps + 1; w++) {
+            if (w == warp) before = sum;
+            sum += bar->warp_sum[w];
+        }
+        *all = sum;
+        return v + before;
     };
-    long long first_count = 0, sum = 0;
+    long long total = 0, mine = 0, incl = 0;
     for (int i0 = 0; i0 < s.seqs; i0 += kScan) {
-        const long long v = seq_tiles(i0 + tid);
-        if (i0 == 0) first_count = v;
-        sum += v;
+        if (i0) __syncthreads();
+        long long all;
+        mine = seq_tiles(i0 + tid);
+        incl = block_incl(mine, &all);
+        total += all;
     }
-    {
-        const long long w = warp_incl(sum);
-        if (tid == 0) bar->total = 0;
-        __syncthreads();
-        if (lane == 31) atomicAdd(&bar->total, (unsigned long long)w);
-        __syncthreads();
-    }
-    const long long total = (long long)bar->total;
     if (total == 0) return;
     const long long want = (total + wk.min_tiles - 1) / wk.min_tiles;
     const int parts = (int)(want < (long long)gridDim.x ? want : (long long)gridDim.x);
@@ -186,19 +204,17 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     {
         long long base = 0;
         for (int i0 = 0; i0 < s.seqs; i0 += kScan) {
-            const long long v = i0 == 0 ? first_count : seq_tiles(i0 + tid);
-            const long long incl = warp_incl(v);
-            __syncthreads();
-            long long* ws = reinterpret_cast<long long*>(buf);
-            if (lane == 31) ws[warp] = incl;
-            __syncthreads();
-            long long before = base;
-            for (int w = 0; w < warp; w++) before += ws[w];
-            if (x0 >= before + incl - v && x0 < before + incl) {
-                bar->seq = i0 + tid;
-                bar->item_start = before + incl - v;
+            long long all = 0;
+            if (s.seqs > kScan) {             // (the one chunk of a smaller batch is still in registers)
+                __syncthreads();
+                mine = seq_tiles(i0 + tid);
+                incl = block_incl(mine, &all);
             }
-            for (int w = 0; w < C::kWarps + 1; w++) base += ws[w];
+            if (x0 >= base + incl - mine && x0 < base + incl) {
+                bar->seq = i0 + tid;
+                bar->item_start = base + incl - mine;
+            }
+            base += all;
         }
         __syncthreads();
     }
@@ -208,7 +224,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     int head = 0, blk = 0;
     {
         const long long per_head = attend_seq_tiles(c, s, span, group, RB, a.window);
-        head = (int)((x0 - item) / per_head);
+        head = (int)(attend_div(x0 - item, per_head));
         item += head * per_head;
     }
     int nblk = attend_blocks(span, group, RB);
@@ -231,6 +247,9 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         }
         b = attend_block(c, s, span, group, RB, a.window, blk);
     };
+    // query row r of the block is (new token, query head of the group); rem0 + r < group + 64, so the reciprocal is exact
+    auto token_of = [&](int r) { return b.j0 + (int)(((unsigned)(b.r0 - b.j0 * group + r) * wk.group_recip) >> 32); };
+    auto head_of = [&](int r) { return b.r0 + r - token_of(r) * group; };
     bool dead = false;                        // a wait ran out: wait for nothing more, finish the launch
     auto wait = [&](uint64_t* which, uint32_t parity, int code) {
         if (dead || mbar_wait(which, parity)) return;
@@ -243,9 +262,18 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         const int box = kv_min(kAttendTile, 1 << c.page_shift), pp = kAttendTile / box;
         const int copies = pp * (D / 64) * 2;
         const int piece = lane % pp, half = (lane / pp) % (D / 64), which = lane / (pp * (D / 64));
-        int n = 0;
+        int n = 0, nq = 0;
         for (; item < x1; advance()) {
             const int ta = item < x0 ? (int)(x0 - item) : 0, tb = item + b.tiles > x1 ? (int)(x1 - item) : b.tiles;
+            // the block's q rows come before its tiles, so that they are not queued behind a ring full of them
+            if (nq > 0) wait(&bar->q_empty, (nq - 1) & 1, 42);
+            nq++;
+            if (lane == 0) mbar_expect_tx(&bar->q_full, (uint32_t)b.rows * D * 4);
+            __syncwarp();
+            for (int r = lane; r < b.rows; r += 32) {
+                const int j = token_of(r), h = head * group + head_of(r);
+                bulk_g2s(qrow + r * C::kPitch, a.q + (size_t)(span.first + j) * a.ldq + (size_t)h * D, D * 4, &bar->q_full);
+            }
             for (int t = ta; t < tb; t++, n++) {
                 const int st = n % C::kStages;
                 const int pos = (b.t0 + t) * kAttendTile + piece * box;
@@ -270,43 +298,32 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 
     // ---- consumers
     const int wm = warp % WM, kn = warp / WM, g = lane >> 2, t4 = lane & 3;
-    constexpr int kCons = 32 * C::kWarps;
     const uint32_t ring_addr = smem_u32(ring);
     const uint32_t k_lane = (uint32_t)((kn * C::kKeys + ((lane >> 4) & 1) * 8 + (lane & 7)) * 128);
     const uint32_t v_lane = (uint32_t)((kn * C::kKeys + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128);
     const int box_shift = kv_min(6, c.page_shift);
-    int n = 0;
+    int n = 0, nq = 0;
     for (; item < x1; advance()) {
         const int ta = item < x0 ? (int)(x0 - item) : 0, tb = item + b.tiles > x1 ? (int)(x1 - item) : b.tiles;
 
-        // q of the block's rows, rotated and scaled to log2 units, into `buf`; a pair of elements per thread and row, its
-        // angle kept while the token stays the same (the query heads of a group)
-        named_bar_sync(1, kCons);
+        // q of the block's rows, rotated and scaled to log2 units in place; a pair of elements per thread and row, its angle
+        // kept while the token stays the same (the query heads of a group)
+        wait(&bar->q_full, nq & 1, 43);
+        nq++;
         {
-            constexpr int kPairs = D / 2, kStep = kCons / kPairs > 0 ? kCons / kPairs : 1;
+            constexpr int kStep = kCons / kPairs;
             const float scale = a.scale * kLog2e;
-            for (int p = tid % kPairs; p < kPairs; p += kCons) {
-                const bool rot = 2 * p < rope.rotary;
-                const int e0 = rot && !rope.interleaved ? p : 2 * p, e1 = rot && !rope.interleaved ? p + (rope.rotary >> 1) : 2 * p + 1;
-                const double turns = rot ? rope.turns[p] : 0.0;
-                int jt = -1;
-                float cs = 1.0f, sn = 0.0f;
+            int jt = -1;
+            float cs = 1.0f, sn = 0.0f;
 #pragma unroll 4
-                for (int r = tid / kPairs; r < RB; r += kStep) {
-                    float x = 0.0f, y = 0.0f;
-                    if (r < b.rows) {
-                        const int j = (b.r0 + r) / group, h = head * group + (b.r0 + r) % group;
-                        const float* q = a.q + (size_t)(span.first + j) * a.ldq + (size_t)h * D;
-                        x = q[e0];
-                        y = q[e1];
-                        if (rot && j != jt) {
-                            rope_cos_sin(turns, span.pos(j), &cs, &sn);
-                            jt = j;
-                        }
-                    }
-                    buf[r * C::kPitch + e0] = fmaf(-y, sn, x * cs) * scale;
-                    buf[r * C::kPitch + e1] = fmaf(y, cs, x * sn) * scale;
-                }
+            for (int r = tid / kPairs; r < RB; r += kStep) {
+                float* q = qrow + r * C::kPitch;
+                const int j = token_of(r);
+                if (rot && j != jt && r < b.rows) rope_cos_sin(turns, span.pos(j), &cs, &sn);
+                jt = j;
+                const float x = q[e0], y = q[e1];
+                q[e0] = fmaf(-y, sn, x * cs) * scale;
+                q[e1] = fmaf(y, cs, x * sn) * scale;
             }
         }
         named_bar_sync(1, kCons);
@@ -314,7 +331,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         float unscale = 1.0f;
         uint32_t qa[C::kQSmem ? 1 : KS][4], qb[C::kQSmem || !BF ? 1 : KS][2];
         {
-            const float* q = buf + (wm * 8 + g) * C::kPitch;
+            const float* q = qrow + (wm * 8 + g) * C::kPitch;
             float qscale = 1.0f;
             if (!BF) {
                 float mx = 0.0f;
@@ -348,10 +365,16 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 }
             }
         }
+        auto q_done = [&] {   // the next block's q may land (by the async proxy, behind this thread's own writes)
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->q_empty);
+        };
+        if constexpr (!C::kOneBuf) q_done();
         if constexpr (C::kQSmem) named_bar_sync(1, kCons);
 
         // keys this thread's row sees, and those that every row of the block sees
-        const int my_r = wm * 8 + g, my_j = (b.r0 + my_r) / group;
+        const int my_r = wm * 8 + g, my_j = token_of(my_r);
         const int lo_r = my_r < b.rows ? kv_seen_lo(span.pos(my_j), a.window) : 0;
         const int hi_r = my_r < b.rows ? kv_seen_hi(c, s, span.pos(my_j)) : 0;
         const int lo_all = kv_seen_lo(span.pos(b.j1), a.window), hi_all = kv_seen_hi(c, s, span.pos(b.j0));
@@ -488,29 +511,41 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         // the warps that share rows: pairwise through `buf`, in a fixed order
         named_bar_sync(1, kCons);
         const bool tainted = bar->tainted != 0;
+        auto give = [&](float* slot) {
 #pragma unroll
-        for (int half = WN / 2; half > 0; half >>= 1) {
-            float* slot = buf + (size_t)((kn % half) * WM + wm) * (8 * D + 32);
-            if (kn >= half && kn < 2 * half) {
+            for (int i = 0; i < NT; i++) *reinterpret_cast<float2*>(slot + i * 64 + lane * 2) = oo[i];
+            if (t4 == 0) *reinterpret_cast<float2*>(slot + 8 * D + 2 * g) = make_float2(m, l);
+        };
+        auto take = [&](const float* slot) {
+            const float2 ml = *reinterpret_cast<const float2*>(slot + 8 * D + 2 * g);
+            const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.0f : mn;
+            const float f0 = ex2f(m - base), f1 = ex2f(ml.x - base);
+            l = l * f0 + ml.y * f1;
+            m = mn;
 #pragma unroll
-                for (int i = 0; i < NT; i++) *reinterpret_cast<float2*>(slot + i * 64 + lane * 2) = oo[i];
-                if (t4 == 0) *reinterpret_cast<float2*>(slot + 8 * D + 2 * g) = make_float2(m, l);
+            for (int i = 0; i < NT; i++) {
+                const float2 w = *reinterpret_cast<const float2*>(slot + i * 64 + lane * 2);
+                oo[i].x = oo[i].x * f0 + w.x * f1;
+                oo[i].y = oo[i].y * f0 + w.y * f1;
             }
-            named_bar_sync(1, kCons);
-            if (kn < half) {
-                const float2 ml = *reinterpret_cast<const float2*>(slot + 8 * D + 2 * g);
-                const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.0f : mn;
-                const float f0 = ex2f(m - base), f1 = ex2f(ml.x - base);
-                l = l * f0 + ml.y * f1;
-                m = mn;
+        };
+        if constexpr (C::kMerge == 1) {           // one warp at a time, where the buffer holds no more
 #pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    const float2 w = *reinterpret_cast<const float2*>(slot + i * 64 + lane * 2);
-                    oo[i].x = oo[i].x * f0 + w.x * f1;
-                    oo[i].y = oo[i].y * f0 + w.y * f1;
-                }
+            for (int w = 1; w < WN; w++) {
+                if (kn == w) give(buf);
+                named_bar_sync(1, kCons);
+                if (kn == 0) take(buf);
+                if (w + 1 < WN) named_bar_sync(1, kCons);
             }
-            if (half > 1) named_bar_sync(1, kCons);
+        } else {
+#pragma unroll
+            for (int half = WN / 2; half > 0; half >>= 1) {
+                float* slot = buf + ((kn % half) * WM + wm) * C::kSlot;
+                if (kn >= half && kn < 2 * half) give(slot);
+                named_bar_sync(1, kCons);
+                if (kn < half) take(slot);
+                if (half > 1) named_bar_sync(1, kCons);
+            }
         }
 
         // rows of results: D sums, then m and l
@@ -525,9 +560,9 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         if (tainted) {
             // A value that some rows of the block see and others do not is not finite: weight 0 does not hide it in a matrix
             // product.  The rows again, one by one and key by key, over this CTA's tiles of the block.
-            float* q = buf + (RB + warp) * C::kPitch;
             for (int r = warp; r < b.rows; r += C::kWarps) {
-                const int j = (b.r0 + r) / group, h = head * group + (b.r0 + r) % group, pos = span.pos(j);
+                float* q = buf + r * C::kPitch;   // the row's results make room for its q, and come again
+                const int j = token_of(r), h = head * group + head_of(r), pos = span.pos(j);
                 const float* src = a.q + (size_t)(span.first + j) * a.ldq + (size_t)h * D;
                 __syncwarp();
                 for (int e = lane; e < D; e += 32) q[e] = rope_element(rope, src, e, pos) * (a.scale * kLog2e);
@@ -535,17 +570,17 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 float pm, pl, acc[D / 32];
                 attend_row_plain<T, D>(c, s, seq, head, q, kv_max(kv_seen_lo(pos, a.window), (b.t0 + ta) * kAttendTile),
                                        kv_min(kv_seen_hi(c, s, pos), (b.t0 + tb) * kAttendTile), lane, &pm, &pl, acc);
-                float* row = buf + r * C::kPitch;
+                __syncwarp();
 #pragma unroll
-                for (int e = 0; e < D / 32; e++) row[lane + 32 * e] = acc[e];
-                if (lane == 0) *reinterpret_cast<float2*>(row + D) = make_float2(pm, pl);
+                for (int e = 0; e < D / 32; e++) q[lane + 32 * e] = acc[e];
+                if (lane == 0) *reinterpret_cast<float2*>(q + D) = make_float2(pm, pl);
             }
             named_bar_sync(1, kCons);
             if (tid == 0) bar->tainted = 0;
         }
 
         auto store = [&](int r, int e, float4 v, float inv) {   // elements e .. e + 3 of row r of the block
-            const int j = (b.r0 + r) / group, h = head * group + (b.r0 + r) % group;
+            const int j = token_of(r), h = head * group + head_of(r);
             const size_t at = (size_t)(span.first + j) * a.ldo + (size_t)h * D + e;
             v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
             if (a.out_bf16) {
@@ -563,16 +598,15 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 const float sum = row[D + 1];
                 store(r, e, *reinterpret_cast<const float4*>(row + e), sum == 0.0f ? 0.0f : 1.0f / sum);
             }
+            if constexpr (C::kOneBuf) q_done();
             continue;
         }
         // A piece.  A CTA has at most two: one of a block begun before its run (slot 0), one of a block that goes on behind
         // it (slot 1); the block's ticket belongs to the CTA it begins in.
         const int c0 = attend_part_of(total, parts, item), c1 = attend_part_of(total, parts, item + b.tiles - 1), np = c1 - c0 + 1;
-        auto piece_of = [&](int cta) {
-            return wk.pieces + ((size_t)cta * 2 + (item >= attend_cut(total, parts, cta) ? 1 : 0)) * C::kPieceFloats;
-        };
+        auto piece_of = [&](int p) { return wk.pieces + ((size_t)(c0 + p) * 2 + (p == 0 ? 1 : 0)) * C::kPieceFloats; };
         {
-            float4* dst = reinterpret_cast<float4*>(piece_of(blockIdx.x));
+            float4* dst = reinterpret_cast<float4*>(piece_of((int)blockIdx.x - c0));
             for (int i = tid; i < RB * C::kPitch / 4; i += kCons) dst[i] = reinterpret_cast<const float4*>(buf)[i];
         }
         named_bar_sync(1, kCons);
@@ -584,7 +618,10 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             __threadfence();
         }
         named_bar_sync(1, kCons);
-        if (!bar->last) continue;
+        if (!bar->last) {
+            if constexpr (C::kOneBuf) q_done();
+            continue;
+        }
         // The join: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i, pieces in order; their (m, l) come through `buf`, as
         // many at a time as it holds.
         constexpr int kFit = C::kBufFloats / (2 * RB), NV = RB * D / 4 / kCons;
@@ -601,7 +638,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             const int pn = kv_min(kFit, np - p0);
             named_bar_sync(1, kCons);
             for (int i = tid; i < pn * RB; i += kCons)
-                ml[i] = __ldcg(reinterpret_cast<const float2*>(piece_of(c0 + p0 + i / RB) + (i % RB) * C::kPitch + D));
+                ml[i] = __ldcg(reinterpret_cast<const float2*>(piece_of(p0 + i / RB) + (i % RB) * C::kPitch + D));
             named_bar_sync(1, kCons);
 #pragma unroll
             for (int v = 0; v < NV; v++) {
@@ -614,7 +651,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 M[v] = mn;
 #pragma unroll 8
                 for (int p = 0; p < pn; p++) {
-                    const float4 w = __ldcg(reinterpret_cast<const float4*>(piece_of(c0 + p0 + p) + r * C::kPitch + e));
+                    const float4 w = __ldcg(reinterpret_cast<const float4*>(piece_of(p0 + p) + r * C::kPitch + e));
                     const float2 x = ml[p * RB + r];
                     const float f = ex2f(x.x - base);
                     L[v] = fmaf(x.y, f, L[v]);
@@ -630,6 +667,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             const int i = tid + v * kCons, r = i / (D / 4), e = 4 * (i % (D / 4));
             if (r < b.rows) store(r, e, acc[v], L[v] == 0.0f ? 0.0f : 1.0f / L[v]);
         }
+        if constexpr (C::kOneBuf) q_done();
     }
 }
 
@@ -677,6 +715,7 @@ int32_t encode_cache(CUtensorMap* map, const KvCacheView& c, void* base, const v
 }
 
 namespace {
+constexpr int kSplitMinTiles = 2;
 constexpr size_t kTicketBytes = 8192;   // [2 x SMs]
 
 template <typename T, int D, int WM>
@@ -704,7 +743,8 @@ int32_t launch_split(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s,
     wk.tickets = reinterpret_cast<unsigned*>(ws);
     wk.pieces = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + kTicketBytes);
     wk.status = gemm_status_word();
-    wk.min_tiles = 1;
+    wk.min_tiles = kSplitMinTiles;
+    wk.group_recip = (0x100000000ull + (unsigned)(a.heads / c.heads) - 1) / (unsigned)(a.heads / c.heads);
     FERRIC_CUDA_TRY(launch_kernel(attend_split_kernel<T, D, WM>, dim3((unsigned)(tune.sm_count * C::kMinCtas)), dim3(C::kThreads), C::kSmem, st,
                                   tune.pdl, kmap, vmap, c, s, r, a, wk));
     return kOk;

@@ -262,7 +262,7 @@ int32_t ferric_cuda_kv_attend(ferric_cuda_ctx* ctx, const ferric_kv_cache* cache
     AttendArgs a;
     int32_t rc;
     if ((rc = cache_view(cache, &c)) != kOk || (rc = seqs_view(seqs, c, n_tokens, &s)) != kOk) return rc;
-    if (n_q_heads == 0 || n_q_heads % cache->n_heads != 0 || n_q_heads > 65536) {
+    if (n_q_heads == 0 || n_q_heads % cache->n_heads != 0 || n_q_heads > 16384) {
         set_last_error("%zu query heads over %zu key-value heads", n_q_heads, cache->n_heads);
         return kErrShape;
     }

@@ -137,16 +137,21 @@ FERRIC_KV_HD long long attend_seq_tiles(const KvCacheView& c, const KvSeqsView& 
     for (int b = 0; b < nb; b++) t += attend_block(c, s, p, group, rb, window, b).tiles;
     return t;
 }
+// 64-bit quotient; nearly always both fit 32 bits, where the division costs a fraction
+FERRIC_KV_HD long long attend_div(long long a, long long b)
+{
+    return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
 // `total` tiles over `parts` CTAs: part i starts at attend_cut(i), and tile x is attend_part_of(x)'s.
 FERRIC_KV_HD long long attend_cut(long long total, int parts, int i)
 {
-    const long long q = total / parts, r = total % parts;
+    const long long q = attend_div(total, parts), r = total - q * parts;
     return i * q + (i < r ? i : r);
 }
 FERRIC_KV_HD int attend_part_of(long long total, int parts, long long x)
 {
-    const long long q = total / parts, r = total % parts;
-    return (int)(x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q);
+    const long long q = attend_div(total, parts), r = total - q * parts;
+    return (int)(x < r * (q + 1) ? attend_div(x, q + 1) : r + attend_div(x - r * (q + 1), q));
 }
 
 }  // namespace ferric
