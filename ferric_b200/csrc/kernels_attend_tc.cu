@@ -34,7 +34,14 @@ struct PromptCfg {
     static constexpr int kRows = 128 * kTilesQ;
     static constexpr int kKeys = D == 256 ? 64 : 128;      // keys of a tile
     static constexpr int kSoftWarps = 4 * kTilesQ;
-    static constexpr int kThreads = 32 * (kSoftWarps + 2);
+    // Issuing threads: the MMA queue is shallow, so a thread's barrier waits and commits (about 1000 cycles a unit, beside 58
+    // for each of its 16 or 24 MMAs) leave the tensor pipe idle.  One thread per row tile, in turns: one waits and commits
+    // while the other issues.  (Without turns the two tiles fall into step, products and softmax no longer overlap.)
+    static constexpr int kMmaWarps = kTilesQ;
+    // Two row tiles make three warpgroups of 168 registers a thread; the softmax's 128 scores a row want more, the issuing and
+    // loading warps less, so they trade (2 x 128 x 208 + 128 x 88 = 384 x 168).
+    static constexpr bool kTrade = kTilesQ == 2;
+    static constexpr int kThreads = kTrade ? 384 : 32 * (kSoftWarps + kMmaWarps + 1);
     static constexpr int kQBytes = kTilesQ * kParts * 128 * D * 2;
     static constexpr int kStageBytes = kKeys * D * 2;      // a tile of K or of V
     static constexpr int kFixed = 1024 + 512 + kQBytes;
@@ -49,7 +56,7 @@ constexpr float kPromptShiftF16 = 8.0f;   // f16 weights are scaled by 2^8: at m
 
 struct PromptBars {
     uint64_t full[8], empty[8];
-    uint64_t s_full[2], p_full[2], pv_done[2];
+    uint64_t s_full[2], p_full[2], pv_done[2], turn[2];
     uint32_t tmem;
     int tainted;
 };
@@ -101,6 +108,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v)
         "r"(v[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+                 "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
 // The loads issued before are complete; their registers must not be used earlier, which the empty statements pin down.
 template <int N>
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[N])
@@ -126,6 +140,62 @@ __device__ __forceinline__ float ex2_approx(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// 2^x for a pair, x at most 127: x = n + f with n the nearest whole number (adding 1.5 * 2^23 leaves it in the low bits) and
+// |f| <= 1/2, 2^f by the polynomial of degree 4 whose largest relative error there is least (Remez exchange in 64 bits;
+// 2.7e-6 evaluated in floats, a 700th of what the weights are rounded to in bf16 and a 90th in f16), times 2^n.  Below
+// 2^-126 the weight is 2^-126.  A NaN stays one.
+__device__ __forceinline__ void ex2_poly2(uint64_t x, float& p0, float& p1)
+{
+    float a, b;
+    unpack_f32x2(x, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.0f));
+    x = pack_f32x2(a, b);
+    const uint64_t magic = pack_f32x2(12582912.0f, 12582912.0f), minus_magic = pack_f32x2(-12582912.0f, -12582912.0f);
+    const uint64_t t = add_f32x2(x, magic), n = add_f32x2(t, minus_magic);
+    const uint64_t f = fma_f32x2(n, pack_f32x2(-1.0f, -1.0f), x);
+    uint64_t y = fma_f32x2(f, pack_f32x2(0.00957010191f, 0.00957010191f), pack_f32x2(0.0559178603f, 0.0559178603f));
+    y = fma_f32x2(y, f, pack_f32x2(0.240247448f, 0.240247448f));
+    y = fma_f32x2(y, f, pack_f32x2(0.693121815f, 0.693121815f));
+    y = fma_f32x2(y, f, pack_f32x2(0.999999261f, 0.999999261f));
+    float ta, tb, ya, yb;
+    unpack_f32x2(t, ta, tb);
+    unpack_f32x2(y, ya, yb);
+    // low bits of t: n; 2^n as a float has n + 127 in its exponent field
+    p0 = ya * __int_as_float(__float_as_int(ta) * (1 << 23) + 0x3f800000);
+    p1 = yb * __int_as_float(__float_as_int(tb) * (1 << 23) + 0x3f800000);
+}
+template <int N>
+__device__ __forceinline__ void regs_more()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_fewer()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 template <typename T, int D>
@@ -169,12 +239,13 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     if (tid == 0) {
         for (int i = 0; i < C::kStages; i++) {
             mbar_init(&bar->full[i], 1);
-            mbar_init(&bar->empty[i], 1);
+            mbar_init(&bar->empty[i], C::kMmaWarps);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&bar->s_full[i], 1);
             mbar_init(&bar->p_full[i], 4);
             mbar_init(&bar->pv_done[i], 1);
+            mbar_init(&bar->turn[i], 1);
         }
         bar->tainted = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -196,33 +267,42 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 for (int i = 0; i < 8; i++) rope_cos_sin(rope.turns[8 * u + i], pos, &cs[i], &sn[i]);
             }
             const int g0 = kv_max(0, b.r0 - j * group), g1 = kv_min(group, b.r0 + b.rows - j * group);
-            for (int g = g0; g < g1; g++) {
-                const float* q = a.q + (size_t)(span.first + j) * a.ldq + (size_t)(head * group + g) * D;
-                float x[16];
-                *reinterpret_cast<float4*>(x) = ld_act(reinterpret_cast<const float4*>(q + ea));
-                *reinterpret_cast<float4*>(x + 4) = ld_act(reinterpret_cast<const float4*>(q + ea + 4));
-                *reinterpret_cast<float4*>(x + 8) = ld_act(reinterpret_cast<const float4*>(q + eb));
-                *reinterpret_cast<float4*>(x + 12) = ld_act(reinterpret_cast<const float4*>(q + eb + 4));
-                if (rot) rope_rotate16(x, cs, sn, rope.interleaved);
-                const int row = j * group + g - b.r0, tile = row >> 7, rr = row & 127;
-                uint8_t* base = qs + tile * (C::kParts * 128 * D * 2) + rr * 128;
+            // four heads' loads in flight at a time: a block starts with little else to do
+            constexpr int kAhead = 4;
+            for (int g4 = g0; g4 < g1; g4 += kAhead) {
+                float x[kAhead][16];
 #pragma unroll
-                for (int i = 0; i < 16; i++) x[i] *= scale;
+                for (int i = 0; i < kAhead; i++) {
+                    const float* q = a.q + (size_t)(span.first + j) * a.ldq + (size_t)(head * group + kv_min(g4 + i, g1 - 1)) * D;
+                    *reinterpret_cast<float4*>(x[i]) = ld_act(reinterpret_cast<const float4*>(q + ea));
+                    *reinterpret_cast<float4*>(x[i] + 4) = ld_act(reinterpret_cast<const float4*>(q + ea + 4));
+                    *reinterpret_cast<float4*>(x[i] + 8) = ld_act(reinterpret_cast<const float4*>(q + eb));
+                    *reinterpret_cast<float4*>(x[i] + 12) = ld_act(reinterpret_cast<const float4*>(q + eb + 4));
+                }
 #pragma unroll
-                for (int part = 0; part < C::kParts; part++) {
-                    uint32_t w[8];
+                for (int i = 0; i < kAhead; i++) {
+                    if (g4 + i >= g1) break;
+                    if (rot) rope_rotate16(x[i], cs, sn, rope.interleaved);
+                    const int row = j * group + g4 + i - b.r0, tile = row >> 7, rr = row & 127;
+                    uint8_t* base = qs + tile * (C::kParts * 128 * D * 2) + rr * 128;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        w[i] = pack2<BF>(x[2 * i], x[2 * i + 1]);
-                        if (BF) {
-                            x[2 * i] -= __uint_as_float(w[i] << 16);
-                            x[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+                    for (int e = 0; e < 16; e++) x[i][e] *= scale;
+#pragma unroll
+                    for (int part = 0; part < C::kParts; part++) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            w[e] = pack2<BF>(x[i][2 * e], x[i][2 * e + 1]);
+                            if (BF) {
+                                x[i][2 * e] -= __uint_as_float(w[e] << 16);
+                                x[i][2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+                            }
                         }
+                        uint8_t* p = base + part * (128 * D * 2);
+                        const int ca = ea >> 3, cb = eb >> 3;
+                        *reinterpret_cast<uint4*>(p + (ca >> 3) * (128 * 128) + (((ca & 7) ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4*>(p + (cb >> 3) * (128 * 128) + (((cb & 7) ^ (rr & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
                     }
-                    uint8_t* p = base + part * (128 * D * 2);
-                    const int ca = ea >> 3, cb = eb >> 3;
-                    *reinterpret_cast<uint4*>(p + (ca >> 3) * (128 * 128) + (((ca & 7) ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    *reinterpret_cast<uint4*>(p + (cb >> 3) * (128 * 128) + (((cb & 7) ^ (rr & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
                 }
             }
         }
@@ -248,7 +328,9 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     // keys every row of the block sees: tiles inside need no mask
     const int lo_all = kv_seen_lo(span.pos(b.j1), a.window), hi_all = kv_seen_hi(c, s, span.pos(b.j0));
 
-    if (warp == C::kSoftWarps + 1) {
+    if (warp >= C::kSoftWarps) {
+    if constexpr (C::kTrade) regs_fewer<88>();
+    if (warp == C::kSoftWarps + C::kMmaWarps) {
         // ---- loader: K0 (.. K1), then V_j and K_{j + PRE} in turn, the order in which the products first use them
         const int box = kv_min(kAttendTile, 1 << c.page_shift), pp = KT / box, copies = pp * H;
         const int piece = lane % pp, half = (lane / pp) % H;
@@ -287,70 +369,97 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 __syncwarp();
             }
         }
-    } else if (warp == C::kSoftWarps) {
-        // ---- products.  Unit u = (key tile u / NX, row tile u % NX), S buffer u & 1.
+    } else if (warp < C::kSoftWarps + C::kMmaWarps) {
+        // ---- products of one row tile: unit j is key tile j.  Its S buffer is the tile's own, or, where one tile fills tensor
+        // memory, they alternate; PRE units are issued ahead.  Ring positions: K_j and V_j in the loader's order.
+        const int x = warp - C::kSoftWarps;
         const uint32_t qbase = smem_u32(qs), rbase = smem_u32(ring);
-        const int units = tiles * NX;
         constexpr uint32_t id_s = attend_idesc(BF, KT, false), id_o = attend_idesc(BF, D, true);
         int n = 0;                            // ring position
-        int k_st = 0, v_st = 0;
-        auto issue_s = [&](int u) {
-            const int x = u % NX;
-            if (x == 0) {
-                k_st = n % C::kStages;
-                wait(&bar->full[k_st], (n / C::kStages) & 1, 52);
-                n++;
-            }
-            tc_fence_after();
-            if (lane == 0 && !dead) {
-                const uint32_t kb = umma_desc_lo(rbase + k_st * C::kStageBytes);
-#pragma unroll
-                for (int part = 0; part < C::kParts; part++) {
-                    const uint32_t qb = umma_desc_lo(qbase + (x * C::kParts + part) * (128 * D * 2));
-#pragma unroll
-                    for (int ks = 0; ks < D / 16; ks++)
-                        umma_f16_lo(tmem + (u & 1) * KT, qb + (ks >> 2) * (128 * 128 / 16) + (ks & 3) * 2, kb + (ks >> 2) * (KT * 128 / 16) + (ks & 3) * 2,
-                                    id_s, part > 0 || ks > 0);
-                }
-                if (x == NX - 1) umma_commit(&bar->empty[k_st]);
-                umma_commit(&bar->s_full[u & 1]);
-            }
-            __syncwarp();
+        auto buffer = [&](int j) { return (j * NX + x) & 1; };
+        auto next_stage = [&](int code) {     // the next tile of the ring, landed
+            const int st = n % C::kStages;
+            wait(&bar->full[st], (n / C::kStages) & 1, code);
+            n++;
+            return st;
         };
-        for (int u = 0; u < kv_min(2, units); u++) issue_s(u);
-        for (int u = 0; u < units; u++) {
-            const int x = u % NX, j = u / NX;
-            if (x == 0) {
-                v_st = n % C::kStages;
-                wait(&bar->full[v_st], (n / C::kStages) & 1, 53);
-                n++;
-                // keys outside what any row sees have weight 0; their values must not be infinities or NaN
-                const int k0 = (t0 + j) * KT, z0 = kv_max(0, b.lo - k0), z1 = kv_min(KT, b.hi - k0);
-                if (z0 > 0 || z1 < KT) {
-                    for (int i = lane; i < KT * (D / 8); i += 32) {
-                        const int row = (i >> 3) % KT, hf = i / (8 * KT);
-                        if (row < z0 || row >= z1)
-                            *reinterpret_cast<uint4*>(ring + v_st * C::kStageBytes + hf * (KT * 128) + row * 128 + ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async();
-                    __syncwarp();
-                }
-            }
-            wait(&bar->p_full[u & 1], (u >> 1) & 1, 54);
+        // MMAs are issued in blocks, tile 0's and tile 1's in turn; block i of tile 0 follows block i - 1 of tile 1
+        int block = 0;
+        auto my_turn = [&] {
+            if (NX == 2 && (x == 1 || block > 0)) wait(&bar->turn[x], (x == 1 ? block : block - 1) & 1, 58);
+            block++;
             tc_fence_after();
+        };
+        auto pass_turn = [&] {
+            if (NX == 2 && lane == 0) mbar_arrive(&bar->turn[x ^ 1]);
+        };
+        auto mma_s = [&](int j, int st) {
+            const uint32_t kb = umma_desc_lo(rbase + st * C::kStageBytes);
+#pragma unroll
+            for (int part = 0; part < C::kParts; part++) {
+                const uint32_t qb = umma_desc_lo(qbase + (x * C::kParts + part) * (128 * D * 2));
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ks++)
+                    umma_f16_lo(tmem + buffer(j) * KT, qb + (ks >> 2) * (128 * 128 / 16) + (ks & 3) * 2, kb + (ks >> 2) * (KT * 128 / 16) + (ks & 3) * 2,
+                                id_s, part > 0 || ks > 0);
+            }
+        };
+        for (int j = 0; j < kv_min(PRE, tiles); j++) {
+            const int st = next_stage(52);
+            my_turn();
             if (lane == 0 && !dead) {
+                mma_s(j, st);
+                umma_commit(&bar->s_full[buffer(j)]);
+                umma_commit(&bar->empty[st]);
+            }
+            pass_turn();
+            __syncwarp();
+        }
+        for (int j = 0; j < tiles; j++) {
+            const int sv = next_stage(53);
+            // keys outside what any row sees have weight 0; their values must not be infinities or NaN
+            const int k0 = (t0 + j) * KT, z0 = kv_max(0, b.lo - k0), z1 = kv_min(KT, b.hi - k0);
+            if (z0 > 0 || z1 < KT) {
+                for (int i = lane; i < KT * (D / 8); i += 32) {
+                    const int row = (i >> 3) % KT, hf = i / (8 * KT);
+                    if (row < z0 || row >= z1)
+                        *reinterpret_cast<uint4*>(ring + sv * C::kStageBytes + hf * (KT * 128) + row * 128 + ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async();
+                __syncwarp();
+            }
+            const bool more = j + PRE < tiles;
+            const int sk = more ? next_stage(52) : 0;
+            wait(&bar->p_full[buffer(j)], ((j * NX + x) >> 1) & 1, 54);
+            my_turn();
+            if (lane == 0 && !dead) {
+                const uint64_t vd = umma_desc_rows(rbase + sv * C::kStageBytes, KT * 128);
 #pragma unroll
                 for (int kk = 0; kk < KT / 16; kk++)
-                    umma_ts(tmem + C::kOCol + x * D, tmem + (u & 1) * KT + kk * 8, umma_desc_rows(rbase + v_st * C::kStageBytes + kk * 2048, KT * 128), id_o,
-                            j > 0 || kk > 0);
-                if (x == NX - 1) umma_commit(&bar->empty[v_st]);
+                    umma_ts(tmem + C::kOCol + x * D, tmem + buffer(j) * KT + kk * 8, vd + kk * (2048 / 16), id_o, j > 0 || kk > 0);
+                umma_commit(&bar->empty[sv]);   // before S: the tile after next is waiting for this stage
+                if (more) mma_s(j + PRE, sk);
+            }
+            pass_turn();
+            if (lane == 0 && !dead) {
+                if (more) {
+                    umma_commit(&bar->s_full[buffer(j + PRE)]);
+                    umma_commit(&bar->empty[sk]);
+                }
                 umma_commit(&bar->pv_done[x]);
             }
             __syncwarp();
-            if (u + 2 < units) issue_s(u + 2);
         }
+    }
+    // Back to the launch's split, one warpgroup at a time and only when all of its warps are here: a warp without a role that
+    // asked for its registers back early would take what the softmax is waiting for.
+    if constexpr (C::kTrade) {
+        named_bar_sync(1, 128);
+        regs_more<168>();
+    }
     } else {
         // ---- softmax: thread = row
+        if constexpr (C::kTrade) regs_more<208>();
         const int x = warp >> 2, row = x * 128 + (warp & 3) * 32 + lane, r = b.r0 + row;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const int j_tok = r / group;
@@ -364,23 +473,26 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const unsigned valid = __ballot_sync(0xffffffffu, lane < pages && kv_page(c, s, seq, (k0 + (lane << run)) >> c.page_shift) >= 0);
             wait(&bar->s_full[sb], (u >> 1) & 1, 55);
             tc_fence_after();
-            uint32_t w[KT];
+            const uint32_t s_col = tmem + lanes + sb * KT;
+            const bool masked = k0 < lo_all || k0 + KT > hi_all || valid != (1u << pages) - 1u;
+            auto mask = [&](uint32_t* w, int i0, int count) {   // scores of keys this row does not see
 #pragma unroll
-            for (int i = 0; i < KT / 32; i++) tmem_ld32_nowait(tmem + lanes + sb * KT + 32 * i, w + 32 * i);
-            tmem_wait_ld(w);
-            if (k0 < lo_all || k0 + KT > hi_all || valid != (1u << pages) - 1u) {
-#pragma unroll
-                for (int i = 0; i < KT; i++) {
-                    const int key = k0 + i;
-                    const bool page = (valid >> (i >> run)) & 1u;
+                for (int i = 0; i < count; i++) {
+                    const int key = k0 + i0 + i;
+                    const bool page = (valid >> ((i0 + i) >> run)) & 1u;
                     if (!(key >= lo_r && key < hi_r && page)) w[i] = 0xff800000u;   // -inf
                 }
-            }
-            float mx = -INFINITY;
+            };
+            uint32_t w[KT];
+#pragma unroll
+            for (int i = 0; i < KT / 32; i++) tmem_ld32_nowait(s_col + 32 * i, w + 32 * i);
+            tmem_wait_ld(w);
+            if (masked) mask(w, 0, KT);
+            float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < KT; i += 2)
-                asm("max.f32 %0, %0, %1, %2;" : "+f"(mx) : "f"(__uint_as_float(w[i])), "f"(__uint_as_float(w[i + 1])));
-            mx -= kShift;
+                asm("max.f32 %0, %0, %1, %2;" : "+f"(mq[(i >> 1) & 3]) : "f"(__uint_as_float(w[i])), "f"(__uint_as_float(w[i + 1])));
+            const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) - kShift;
             const bool move = mx > m + kSlack || (m == -INFINITY && mx > m);
             if (__any_sync(0xffffffffu, move)) {
                 const float mn = move ? mx : m, fix = move ? ex2_approx(m - mn) : 1.0f;
@@ -402,17 +514,30 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 }
             }
             const float base = m == -INFINITY ? 0.0f : m;
-            float sum0 = 0.0f, sum1 = 0.0f;
+            const uint64_t minus = pack_f32x2(-base, -base);
+            uint64_t sum[2] = {0, 0};
+            // A quarter of the exponentials run as polynomials on the FMA pipe: ex2 retires 4 lanes a cycle and scheduler, and 128
+            // a row and tile would be the loop's bound.
 #pragma unroll
             for (int i = 0; i < KT / 2; i++) {
-                const float p0 = ex2_approx(__uint_as_float(w[2 * i]) - base), p1 = ex2_approx(__uint_as_float(w[2 * i + 1]) - base);
-                sum0 += p0;
-                sum1 += p1;
+                const uint64_t x = add_f32x2(pack_f32x2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])), minus);
+                float p0, p1;
+                if (i % 4 == 3) {
+                    ex2_poly2(x, p0, p1);
+                } else {
+                    unpack_f32x2(x, p0, p1);
+                    p0 = ex2_approx(p0);
+                    p1 = ex2_approx(p1);
+                }
+                sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(p0, p1));
                 w[i] = pack2<BF>(p0, p1);
+                if (i % 16 == 15) tmem_st16(s_col + (i - 15), w + (i - 15));
             }
-            l += sum0 + sum1;
-#pragma unroll
-            for (int i = 0; i < KT / 64; i++) tmem_st32(tmem + lanes + sb * KT + 32 * i, w + 32 * i);
+            {
+                float a0, a1;
+                unpack_f32x2(add_f32x2(sum[0], sum[1]), a0, a1);
+                l += a0 + a1;
+            }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -420,7 +545,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
         wait(&bar->pv_done[x], (tiles - 1) & 1, 57);
         tc_fence_after();
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = m == -INFINITY || l == 0.0f ? 0.0f : 1.0f / l;   // no key seen: zeros, whatever the polynomials' 2^-126 sum to
         __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + j_tok) * a.ldo + (size_t)(head * group + r % group) * D;
 #pragma unroll 1
         for (int i = 0; i < D / 32; i++) {
@@ -439,6 +564,10 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             }
         }
         tc_fence_before();
+        if constexpr (C::kTrade) {
+            named_bar_sync(2 + x, 128);
+            regs_fewer<168>();
+        }
     }
     __syncthreads();
     if (warp == C::kSoftWarps)

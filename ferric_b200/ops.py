@@ -1,7 +1,6 @@
 """Python mirror of the reference's QMatrix / matmul_q operator interface (see package docstring)."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 from typing import Optional
@@ -64,6 +63,7 @@ class Context:
             _check(self._lib.ferric_cuda_ctx_create_on_stream(self.device, C.c_void_p(int(stream)), C.byref(h)),
                    "Context")
         self._h = h
+        self._stream = int(self._lib.ferric_cuda_ctx_stream(h) or 0)
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -78,6 +78,7 @@ class Context:
 
     def set_stream(self, cuda_stream: int) -> None:
         _check(self._lib.ferric_cuda_ctx_set_stream(self._h, C.c_void_p(int(cuda_stream))), "set_stream")
+        self._stream = int(cuda_stream)
 
     def use_torch_stream(self) -> None:
         self.set_stream(torch.cuda.current_stream(self.device).cuda_stream)
@@ -510,6 +511,7 @@ class KVSeqs:
         n, cols = page_table.shape
         self._c = _lib.KvSeqs(page_table.data_ptr(), n, cols, page_table.stride(0) if n > 1 else 0, lens.data_ptr(),
                               starts.data_ptr() if starts is not None else None)
+        self._ref, self._dev = C.byref(self._c), lens.get_device()
 
 
 class KVCache:
@@ -534,6 +536,7 @@ class KVCache:
         self.n_heads, self.page_size, self.head_dim = heads, page, dim
         self._c = _lib.KvCache(k.data_ptr(), v.data_ptr(), GGML_F16 if k.dtype == torch.float16 else GGML_BF16, n_pages, page, heads,
                                dim, k.stride(0) if n_pages > 1 else 0)
+        self._ref, self._dev = C.byref(self._c), ctx.device
 
     @classmethod
     def empty(cls, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
@@ -543,51 +546,50 @@ class KVCache:
         dev = torch.device("cuda", ctx.device)
         return cls(ctx, torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
 
-    def _rows(self, x: torch.Tensor, name: str) -> torch.Tensor:
-        if not x.is_cuda or x.dtype != torch.float32 or x.dim() not in (2, 3):
+    def _rows(self, x: torch.Tensor, name: str):
+        """(x as a matrix the kernels take in place, rows, columns, address, row stride)"""
+        if x.dtype is not torch.float32 or not x.is_cuda:
             raise TypeError(f"{name} must be a float32 CUDA tensor [tokens, heads * head_dim] or [tokens, heads, head_dim]")
+        if x.get_device() != self._dev:
+            raise ValueError(f"{name} is on {x.device}, the context on device {self._dev}")
         if x.dim() == 3:
             if x.shape[2] != self.head_dim:
                 raise ValueError(f"{name} has heads of {x.shape[2]}, the cache of {self.head_dim}")
             x = x.flatten(1) if x.stride(2) == 1 and (x.shape[1] <= 1 or x.stride(1) == self.head_dim) else x.contiguous().flatten(1)
-        if x.device.index != self.ctx.device:
-            raise ValueError(f"{name} is on {x.device}, the context on device {self.ctx.device}")
-        ok = (x.shape[1] <= 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % 4 == 0)) \
-            and x.data_ptr() % 16 == 0
-        return x if ok else x.contiguous()
+        elif x.dim() != 2:
+            raise TypeError(f"{name} must have two or three dimensions, not {x.dim()}")
+        n, cols = x.shape
+        ld, step = x.stride()
+        p = x.data_ptr()
+        if (step != 1 and cols > 1) or (n > 1 and (ld < cols or ld % 4)) or p % 16:
+            x = x.contiguous()
+            ld, p = cols, x.data_ptr()
+        return x, n, cols, p, ld if n > 1 else 0
 
-    @contextlib.contextmanager
-    def _ordered(self):
-        """Where the context's stream is not torch's current one: the call waits for what torch has queued there, and what torch
-        queues next waits for the call, so operands and results may be made and dropped as if it ran on that stream."""
-        st = self._lib.ferric_cuda_ctx_stream(self.ctx._h) or 0
-        cur = torch.cuda.current_stream(self.ctx.device)
-        if st == cur.cuda_stream:
-            yield
+    def _run(self, fn, where: str, *args) -> None:
+        """The call on the context's stream.  Where that is not torch's current one, it waits for what torch has queued there and
+        what torch queues next waits for it, so operands and results may be made and dropped as if it ran on that stream."""
+        st = self.ctx._stream
+        if st == torch._C._cuda_getCurrentRawStream(self._dev):
+            _check(fn(self.ctx._h, self._ref, *args), where)
             return
-        own = torch.cuda.ExternalStream(st, device=self.ctx.device) if st else torch.cuda.default_stream(self.ctx.device)
+        cur = torch.cuda.current_stream(self._dev)
+        own = torch.cuda.ExternalStream(st, device=self._dev) if st else torch.cuda.default_stream(self._dev)
         own.wait_stream(cur)
         try:
-            yield
+            _check(fn(self.ctx._h, self._ref, *args), where)
         finally:
             cur.wait_stream(own)
 
-    def _common(self, seqs: KVSeqs, rope: Optional[Rope]):
-        if seqs.lens.device.index != self.ctx.device:
-            raise ValueError(f"the sequences are on {seqs.lens.device}, the context on device {self.ctx.device}")
-        return C.byref(self._c), C.byref(seqs._c), rope._h if rope is not None else None
-
     def append(self, seqs: KVSeqs, k: torch.Tensor, v: torch.Tensor, rope: Optional[Rope] = None) -> None:
         """Store the new tokens' keys (rotated by ``rope``) and values at their positions (``ferric_cuda_kv_append``)."""
-        k, v = self._rows(k, "k"), self._rows(v, "v")
-        cols = self.n_heads * self.head_dim
-        if k.shape[1] != cols or v.shape != k.shape:
-            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {cols}]")
-        c, s, r = self._common(seqs, rope)
-        n = k.shape[0]
-        with self._ordered():
-            _check(self._lib.ferric_cuda_kv_append(self.ctx._h, c, s, r, k.data_ptr(), k.stride(0) if n > 1 else 0, v.data_ptr(),
-                                                   v.stride(0) if n > 1 else 0, n), "kv_append")
+        k, n, cols, pk, ldk = self._rows(k, "k")
+        v, nv, cols_v, pv, ldv = self._rows(v, "v")
+        if cols != self.n_heads * self.head_dim or cols_v != cols or nv != n:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {self.n_heads * self.head_dim}]")
+        if seqs._dev != self._dev:
+            raise ValueError(f"the sequences are on device {seqs._dev}, the context on device {self._dev}")
+        self._run(self._lib.ferric_cuda_kv_append, "kv_append", seqs._ref, rope._h if rope is not None else None, pk, ldk, pv, ldv, n)
 
     def attend(self, seqs: KVSeqs, q: torch.Tensor, rope: Optional[Rope] = None, scale: Optional[float] = None, window: int = 0,
                out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -595,27 +597,29 @@ class KVCache:
         rotated by ``rope``; each token sees its sequence's keys up to its own position, the last ``window`` of them where
         that is set.  Returns [tokens, heads * head_dim] in ``out_dtype`` (float32, or bfloat16 for the prefill products),
         or fills ``out``; rows of no sequence are left as they were (in a result made here: as the memory was)."""
-        q = self._rows(q, "q")
-        n, cols = q.shape
-        if cols % self.head_dim != 0:
+        q, n, cols, pq, ldq = self._rows(q, "q")
+        if cols % self.head_dim:
             raise ValueError(f"q has {cols} columns, heads have {self.head_dim}")
         if window < 0:
             raise ValueError("window must not be negative")
+        if scale is None:
+            scale = 0.0
+        elif scale == 0.0:
+            raise ValueError("scale must not be 0 (None = 1 / sqrt(head_dim))")
+        if seqs._dev != self._dev:
+            raise ValueError(f"the sequences are on device {seqs._dev}, the context on device {self._dev}")
         if out is None:
             out = torch.empty((n, cols), dtype=out_dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16) or out.device != q.device or \
-                (out.stride(1) != 1 and cols > 1):
-            raise TypeError("out must be a float32 or bfloat16 tensor of q's shape and device with adjacent columns")
-        if out.dtype not in (torch.float32, torch.bfloat16):
-            raise TypeError("out_dtype must be float32 or bfloat16")
-        if scale is not None and scale == 0.0:
-            raise ValueError("scale must not be 0 (None = 1 / sqrt(head_dim))")
-        c, s, r = self._common(seqs, rope)
-        with self._ordered():
-            _check(self._lib.ferric_cuda_kv_attend(self.ctx._h, c, s, r, q.data_ptr(), q.stride(0) if n > 1 else 0, n, cols // self.head_dim,
-                                                   float(scale) if scale is not None else 0.0, int(window), out.data_ptr(),
-                                                   GGML_F32 if out.dtype == torch.float32 else GGML_BF16,
-                                                   out.stride(0) if n > 1 else 0), "kv_attend")
+            ldo = 0
+        else:
+            if out.shape != q.shape or out.device != q.device or (out.stride(1) != 1 and cols > 1):
+                raise TypeError("out must be a tensor of q's shape and device with adjacent columns")
+            ldo = out.stride(0) if n > 1 else 0
+        ty = GGML_F32 if out.dtype is torch.float32 else GGML_BF16
+        if ty == GGML_BF16 and out.dtype is not torch.bfloat16:
+            raise TypeError("the result is float32 or bfloat16")
+        self._run(self._lib.ferric_cuda_kv_attend, "kv_attend", seqs._ref, rope._h if rope is not None else None, pq, ldq, n,
+                  cols // self.head_dim, scale, window, out.data_ptr(), ty, ldo)
         return out
 
 
