@@ -39,11 +39,11 @@ struct SplitCfg {
     static constexpr int kStageBytes = 2 * kAttendTile * D * 2;
     static constexpr bool kQSmem = D == 256;             // 96 registers of q and 128 of output do not fit one thread
     static constexpr int kQBytes = kQSmem ? WM * (D / 16) * 32 * (kBf16 ? 24 : 16) : 0;
-    static constexpr int kPitch = D + 8;                 // floats of a row of q, or of results: D sums, m, l
+    static constexpr int kPitch = D + 8;                 // floats of a row of q, or of results done again: D sums, m, l
     // warps that hand their results over in one round of the merge
     static constexpr int kMerge = kWN == 1 ? 0 : (D == 256 && WM == 1) ? 1 : kWarps / 2;
     static constexpr int kSlot = 8 * D + 32;
-    static constexpr int kBufFloats = kMerge * kSlot > kRows * kPitch ? kMerge * kSlot : kRows * kPitch;   // merge; results; pieces' (m, l)
+    static constexpr int kBufFloats = kMerge * kSlot > kRows * kPitch ? kMerge * kSlot : kRows * kPitch;   // merge; results done again
     // the widest tiles at head_dim 256 keep q and the results in one place: the next block's q comes when this one is done
     static constexpr bool kOneBuf = D == 256 && WM == 4;
     static constexpr int kFixed = 1024 + kQBytes + (kOneBuf ? 0 : kRows * kPitch * 4) + kBufFloats * 4 + 512;
@@ -53,7 +53,8 @@ struct SplitCfg {
     static constexpr int kStagesFit = (kSmemMax - kFixed) / kStageBytes;
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static constexpr int kSmem = kFixed + kStages * kStageBytes;
-    static constexpr int kPieceFloats = kRows * kPitch;
+    static constexpr int kTileFloats = 8 * D + 16;       // a row tile of a piece
+    static constexpr int kPieceFloats = WM * kTileFloats;
     static_assert(kStages >= 2, "a ring of two stages at least");
 };
 constexpr float kPShiftF16 = 14.0f;   // p in f16 parts is scaled by 2^14: parts stay normal down to 2^-28
@@ -548,20 +549,13 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
         }
 
-        // rows of results: D sums, then m and l
-        named_bar_sync(1, kCons);
-        if (kn == 0) {
-            float* row = buf + (wm * 8 + g) * C::kPitch;
-#pragma unroll
-            for (int i = 0; i < NT; i++) *reinterpret_cast<float2*>(row + 8 * i + 2 * t4) = oo[i];
-            if (t4 == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m, l);
-        }
-        named_bar_sync(1, kCons);
+        // now the kn == 0 warps hold their tile's rows: lane (g, t) elements 8 i + 2 t + {0, 1} of row g
         if (tainted) {
             // A value that some rows of the block see and others do not is not finite: weight 0 does not hide it in a matrix
             // product.  The rows again, one by one and key by key, over this CTA's tiles of the block.
+            named_bar_sync(1, kCons);
             for (int r = warp; r < b.rows; r += C::kWarps) {
-                float* q = buf + r * C::kPitch;   // the row's results make room for its q, and come again
+                float* q = buf + r * C::kPitch;   // the row's q, then its results
                 const int j = token_of(r), h = head * group + head_of(r), pos = span.pos(j);
                 const float* src = a.q + (size_t)(span.first + j) * a.ldq + (size_t)h * D;
                 __syncwarp();
@@ -577,97 +571,107 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
             named_bar_sync(1, kCons);
             if (tid == 0) bar->tainted = 0;
+            const float* row = buf + (wm * 8 + g) * C::kPitch;
+#pragma unroll
+            for (int i = 0; i < NT; i++) oo[i] = *reinterpret_cast<const float2*>(row + 8 * i + 2 * t4);
+            m = row[D];
+            l = row[D + 1];
         }
 
-        auto store = [&](int r, int e, float4 v, float inv) {   // elements e .. e + 3 of row r of the block
-            const int j = token_of(r), h = head * group + head_of(r);
-            const size_t at = (size_t)(span.first + j) * a.ldo + (size_t)h * D + e;
-            v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
-            if (a.out_bf16) {
-                __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
-                *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + at) =
-                    make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
-            } else {
-                *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at) = v;
-            }
+        auto out_at = [&](int r, int e) {   // element e of row r of the block
+            return (size_t)(span.first + token_of(r)) * a.ldo + (size_t)(head * group + head_of(r)) * D + e;
         };
         if (ta == 0 && tb == b.tiles) {
-            for (int i = tid; i < b.rows * (D / 4); i += kCons) {
-                const int r = i / (D / 4), e = 4 * (i % (D / 4));
-                const float* row = buf + r * C::kPitch;
-                const float sum = row[D + 1];
-                store(r, e, *reinterpret_cast<const float4*>(row + e), sum == 0.0f ? 0.0f : 1.0f / sum);
+            if (kn == 0 && my_r < b.rows) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const size_t at = out_at(my_r, 2 * t4);
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const float2 v = make_float2(oo[i].x * inv, oo[i].y * inv);
+                    if (a.out_bf16)
+                        *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(a.out) + at + 8 * i) = __floats2bfloat162_rn(v.x, v.y);
+                    else
+                        *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + at + 8 * i) = v;
+                }
             }
-            if constexpr (C::kOneBuf) q_done();
+            if constexpr (C::kOneBuf) {
+                named_bar_sync(1, kCons);
+                q_done();
+            }
             continue;
         }
-        // A piece.  A CTA has at most two: one of a block begun before its run (slot 0), one of a block that goes on behind
-        // it (slot 1); the block's ticket belongs to the CTA it begins in.
+        // A piece, in the lanes' order: per row tile [i][lane] pairs, then m and l of its rows.  A CTA has at most two: one of a
+        // block begun before its run (slot 0), one of a block that goes on behind it (slot 1); the block's ticket belongs to the
+        // CTA it begins in.
         const int c0 = attend_part_of(total, parts, item), c1 = attend_part_of(total, parts, item + b.tiles - 1), np = c1 - c0 + 1;
         auto piece_of = [&](int p) { return wk.pieces + ((size_t)(c0 + p) * 2 + (p == 0 ? 1 : 0)) * C::kPieceFloats; };
-        {
-            float4* dst = reinterpret_cast<float4*>(piece_of((int)blockIdx.x - c0));
-            for (int i = tid; i < RB * C::kPitch / 4; i += kCons) dst[i] = reinterpret_cast<const float4*>(buf)[i];
+        if (kn == 0) {
+            float* dst = piece_of((int)blockIdx.x - c0) + wm * C::kTileFloats;
+#pragma unroll
+            for (int i = 0; i < NT; i++) *reinterpret_cast<float2*>(dst + i * 64 + lane * 2) = oo[i];
+            if (t4 == 0) *reinterpret_cast<float2*>(dst + 8 * D + 2 * g) = make_float2(m, l);
         }
         named_bar_sync(1, kCons);
         if (tid == 0) {
-            __threadfence();
-            const unsigned before = atomicAdd(wk.tickets + c0, 1u);
+            unsigned before;
+            asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(wk.tickets + c0) : "memory");
             bar->last = before == (unsigned)(np - 1);
             if (bar->last) wk.tickets[c0] = 0;
-            __threadfence();
         }
         named_bar_sync(1, kCons);
-        if (!bar->last) {
-            if constexpr (C::kOneBuf) q_done();
-            continue;
-        }
-        // The join: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i, pieces in order; their (m, l) come through `buf`, as
-        // many at a time as it holds.
-        constexpr int kFit = C::kBufFloats / (2 * RB), NV = RB * D / 4 / kCons;
-        float4 acc[NV];
-        float M[NV], L[NV];
-#pragma unroll
+        if constexpr (C::kOneBuf) q_done();
+        if (!bar->last) continue;
+        // The join: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i, pieces in order, rescaled as the maximum grows.  A thread
+        // takes four elements of a row at a time and asks for eight pieces' (m, l) and elements at once: it is trips to L2 that
+        // the join consists of.
+        constexpr int NV = RB * D / 4 / kCons, kAtOnce = 8;
+#pragma unroll 2
         for (int v = 0; v < NV; v++) {
-            acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-            M[v] = -INFINITY;
-            L[v] = 0.0f;
-        }
-        float2* ml = reinterpret_cast<float2*>(buf);
-        for (int p0 = 0; p0 < np; p0 += kFit) {
-            const int pn = kv_min(kFit, np - p0);
-            named_bar_sync(1, kCons);
-            for (int i = tid; i < pn * RB; i += kCons)
-                ml[i] = __ldcg(reinterpret_cast<const float2*>(piece_of(p0 + i / RB) + (i % RB) * C::kPitch + D));
-            named_bar_sync(1, kCons);
+            const int i = tid + v * kCons, tile = i / (2 * D), at = i % (2 * D), r = tile * 8 + (at & 15) / 2, e = (at >> 4) * 8 + (at & 1) * 4;
+            const size_t o_at = (size_t)tile * C::kTileFloats + 4 * at, ml_at = (size_t)tile * C::kTileFloats + 8 * D + ((at & 15) & ~1);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float M = -INFINITY, L = 0.0f;
+            for (int p = 0; p < np; p += kAtOnce) {
+                float4 w[kAtOnce];
+                float2 x[kAtOnce];
 #pragma unroll
-            for (int v = 0; v < NV; v++) {
-                const int i = tid + v * kCons, r = i / (D / 4), e = 4 * (i % (D / 4));
-                float mn = M[v];
-                for (int p = 0; p < pn; p++) mn = fmaxf(mn, ml[p * RB + r].x);
-                const float base = mn == -INFINITY ? 0.0f : mn, fix = ex2f(M[v] - base);
-                acc[v].x *= fix, acc[v].y *= fix, acc[v].z *= fix, acc[v].w *= fix;
-                L[v] *= fix;
-                M[v] = mn;
-#pragma unroll 8
-                for (int p = 0; p < pn; p++) {
-                    const float4 w = __ldcg(reinterpret_cast<const float4*>(piece_of(p0 + p) + r * C::kPitch + e));
-                    const float2 x = ml[p * RB + r];
-                    const float f = ex2f(x.x - base);
-                    L[v] = fmaf(x.y, f, L[v]);
-                    acc[v].x = fmaf(w.x, f, acc[v].x);
-                    acc[v].y = fmaf(w.y, f, acc[v].y);
-                    acc[v].z = fmaf(w.z, f, acc[v].z);
-                    acc[v].w = fmaf(w.w, f, acc[v].w);
+                for (int k = 0; k < kAtOnce; k++) {
+                    const float* piece = piece_of(kv_min(p + k, np - 1));
+                    x[k] = __ldcg(reinterpret_cast<const float2*>(piece + ml_at));
+                    w[k] = __ldcg(reinterpret_cast<const float4*>(piece + o_at));
+                }
+                float mn = M;
+#pragma unroll
+                for (int k = 0; k < kAtOnce; k++) mn = fmaxf(mn, x[k].x);      // (the last piece again past the end)
+                const float base = mn == -INFINITY ? 0.0f : mn, fix = ex2f(M - base);
+                M = mn;
+                acc.x *= fix, acc.y *= fix, acc.z *= fix, acc.w *= fix;
+                L *= fix;
+#pragma unroll
+                for (int k = 0; k < kAtOnce; k++) {
+                    if (p + k < np) {
+                        const float f = ex2f(x[k].x - base);
+                        L = fmaf(x[k].y, f, L);
+                        acc.x = fmaf(w[k].x, f, acc.x);
+                        acc.y = fmaf(w[k].y, f, acc.y);
+                        acc.z = fmaf(w[k].z, f, acc.z);
+                        acc.w = fmaf(w[k].w, f, acc.w);
+                    }
+                }
+            }
+            if (r < b.rows) {
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                const size_t at_out = out_at(r, e);
+                if (a.out_bf16) {
+                    const __nv_bfloat162 y = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), z = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + at_out) =
+                        make_uint2(*reinterpret_cast<const uint32_t*>(&y), *reinterpret_cast<const uint32_t*>(&z));
+                } else {
+                    *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at_out) =
+                        make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
                 }
             }
         }
-#pragma unroll
-        for (int v = 0; v < NV; v++) {
-            const int i = tid + v * kCons, r = i / (D / 4), e = 4 * (i % (D / 4));
-            if (r < b.rows) store(r, e, acc[v], L[v] == 0.0f ? 0.0f : 1.0f / L[v]);
-        }
-        if constexpr (C::kOneBuf) q_done();
     }
 }
 
