@@ -624,51 +624,69 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         // The join: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i, pieces in order, rescaled as the maximum grows.  A thread
         // takes four elements of a row at a time and asks for eight pieces' (m, l) and elements at once: it is trips to L2 that
         // the join consists of.
-        constexpr int NV = RB * D / 4 / kCons, kAtOnce = 8;
-#pragma unroll 2
-        for (int v = 0; v < NV; v++) {
-            const int i = tid + v * kCons, tile = i / (2 * D), at = i % (2 * D), r = tile * 8 + (at & 15) / 2, e = (at >> 4) * 8 + (at & 1) * 4;
-            const size_t o_at = (size_t)tile * C::kTileFloats + 4 * at, ml_at = (size_t)tile * C::kTileFloats + 8 * D + ((at & 15) & ~1);
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float M = -INFINITY, L = 0.0f;
+        constexpr int NV = RB * D / 4 / kCons, kAtOnce = 8, kPair = NV >= 2 ? 2 : 1;
+#pragma unroll 1
+        for (int v0 = 0; v0 < NV; v0 += kPair) {
+            float4 acc[kPair];
+            float M[kPair], L[kPair];
+            size_t o_at[kPair], ml_at[kPair];
+#pragma unroll
+            for (int v = 0; v < kPair; v++) {
+                const int i = tid + (v0 + v) * kCons, tile = i / (2 * D), at = i % (2 * D);
+                o_at[v] = (size_t)tile * C::kTileFloats + 4 * at;
+                ml_at[v] = (size_t)tile * C::kTileFloats + 8 * D + ((at & 15) & ~1);
+                acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+                M[v] = -INFINITY;
+                L[v] = 0.0f;
+            }
+#pragma unroll 1
             for (int p = 0; p < np; p += kAtOnce) {
-                float4 w[kAtOnce];
-                float2 x[kAtOnce];
+                float4 w[kPair][kAtOnce];
+                float2 x[kPair][kAtOnce];
 #pragma unroll
                 for (int k = 0; k < kAtOnce; k++) {
                     const float* piece = piece_of(kv_min(p + k, np - 1));
-                    x[k] = __ldcg(reinterpret_cast<const float2*>(piece + ml_at));
-                    w[k] = __ldcg(reinterpret_cast<const float4*>(piece + o_at));
+#pragma unroll
+                    for (int v = 0; v < kPair; v++) {
+                        x[v][k] = __ldcg(reinterpret_cast<const float2*>(piece + ml_at[v]));
+                        w[v][k] = __ldcg(reinterpret_cast<const float4*>(piece + o_at[v]));
+                    }
                 }
-                float mn = M;
 #pragma unroll
-                for (int k = 0; k < kAtOnce; k++) mn = fmaxf(mn, x[k].x);      // (the last piece again past the end)
-                const float base = mn == -INFINITY ? 0.0f : mn, fix = ex2f(M - base);
-                M = mn;
-                acc.x *= fix, acc.y *= fix, acc.z *= fix, acc.w *= fix;
-                L *= fix;
+                for (int v = 0; v < kPair; v++) {
+                    float mn = M[v];
 #pragma unroll
-                for (int k = 0; k < kAtOnce; k++) {
-                    if (p + k < np) {
-                        const float f = ex2f(x[k].x - base);
-                        L = fmaf(x[k].y, f, L);
-                        acc.x = fmaf(w[k].x, f, acc.x);
-                        acc.y = fmaf(w[k].y, f, acc.y);
-                        acc.z = fmaf(w[k].z, f, acc.z);
-                        acc.w = fmaf(w[k].w, f, acc.w);
+                    for (int k = 0; k < kAtOnce; k++) mn = fmaxf(mn, x[v][k].x);      // (the last piece again past the end)
+                    const float base = mn == -INFINITY ? 0.0f : mn, fix = ex2f(M[v] - base);
+                    M[v] = mn;
+                    acc[v].x *= fix, acc[v].y *= fix, acc[v].z *= fix, acc[v].w *= fix;
+                    L[v] *= fix;
+#pragma unroll
+                    for (int k = 0; k < kAtOnce; k++) {
+                        if (p + k < np) {
+                            const float f = ex2f(x[v][k].x - base);
+                            L[v] = fmaf(x[v][k].y, f, L[v]);
+                            acc[v].x = fmaf(w[v][k].x, f, acc[v].x);
+                            acc[v].y = fmaf(w[v][k].y, f, acc[v].y);
+                            acc[v].z = fmaf(w[v][k].z, f, acc[v].z);
+                            acc[v].w = fmaf(w[v][k].w, f, acc[v].w);
+                        }
                     }
                 }
             }
-            if (r < b.rows) {
-                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+            for (int v = 0; v < kPair; v++) {
+                const int i = tid + (v0 + v) * kCons, at = i % (2 * D), r = i / (2 * D) * 8 + (at & 15) / 2, e = (at >> 4) * 8 + (at & 1) * 4;
+                if (r >= b.rows) continue;
+                const float inv = L[v] == 0.0f ? 0.0f : 1.0f / L[v];
                 const size_t at_out = out_at(r, e);
                 if (a.out_bf16) {
-                    const __nv_bfloat162 y = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), z = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+                    const __nv_bfloat162 y = __floats2bfloat162_rn(acc[v].x * inv, acc[v].y * inv), z = __floats2bfloat162_rn(acc[v].z * inv, acc[v].w * inv);
                     *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + at_out) =
                         make_uint2(*reinterpret_cast<const uint32_t*>(&y), *reinterpret_cast<const uint32_t*>(&z));
                 } else {
                     *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at_out) =
-                        make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+                        make_float4(acc[v].x * inv, acc[v].y * inv, acc[v].z * inv, acc[v].w * inv);
                 }
             }
         }

@@ -217,8 +217,9 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     pdl_launch_dependents();
     pdl_wait();
 
-    // ---- this CTA's block: blockIdx.y = head, blockIdx.x counts the batch's blocks, each sequence's longest first
-    int seq = 0, blk = (int)blockIdx.x;
+    // ---- this CTA's block: the heads' blocks side by side, each sequence's longest first, so that short ones fill up the end
+    const int head = (int)(blockIdx.x % (unsigned)c.heads);
+    int seq = 0, blk = (int)(blockIdx.x / (unsigned)c.heads);
     KvSpan span{};
     int nb = 0;
     for (; seq < s.seqs; seq++) {
@@ -228,7 +229,6 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         blk -= nb;
     }
     if (seq == s.seqs) return;
-    const int head = blockIdx.y;
     const AttendBlock b = attend_block(c, s, span, group, C::kRows, a.window, nb - 1 - blk);
     const int t0 = b.lo / KT, tiles = kv_max(1, (b.hi + KT - 1) / KT - t0);
 
@@ -608,7 +608,11 @@ int32_t launch_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s
     if ((rc = encode_cache(&kmap, c, c.k, a.q)) != kOk || (rc = encode_cache(&vmap, c, c.v, a.q)) != kOk) return rc;
     // the batch's spans are on the device: as many blocks as any could make, those behind the last return at once
     const long long blocks = ((long long)s.tokens * (a.heads / c.heads)) / C::kRows + s.seqs;
-    FERRIC_CUDA_TRY(launch_kernel(attend_prompt_kernel<T, D>, dim3((unsigned)blocks, (unsigned)c.heads), dim3(C::kThreads), C::kSmem, st, tune.pdl, kmap, vmap,
+    if (blocks * c.heads > INT32_MAX) {
+        set_last_error("%d tokens x %d heads is more than one launch covers", s.tokens, a.heads);
+        return kErrShape;
+    }
+    FERRIC_CUDA_TRY(launch_kernel(attend_prompt_kernel<T, D>, dim3((unsigned)(blocks * c.heads)), dim3(C::kThreads), C::kSmem, st, tune.pdl, kmap, vmap,
                                   c, s, r, a, gemm_status_word()));
     return kOk;
 }
