@@ -227,8 +227,9 @@ int32_t launch_attend(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s
 
 // Many query rows per sequence and a bf16 result: the tcgen05 form (kernels_attend_tc.cu).
 bool attend_prompt_eligible(const KvCacheView& c, const KvSeqsView& s, const AttendArgs& a);
-int32_t launch_attend_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a,
-                             const GemvTuning& tune);
+size_t attend_prompt_ws_bytes(int sm_count);
+int32_t launch_attend_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a, void* ws,
+                             size_t ticket_bytes, const GemvTuning& tune);
 
 // Synchronise the stream and fetch-and-clear the code a GEMM CTA left when one of its bounded waits ran out.
 int32_t gemm_status(cudaStream_t st, int* code);

@@ -738,7 +738,7 @@ int32_t encode_cache(CUtensorMap* map, const KvCacheView& c, void* base, const v
 
 namespace {
 constexpr int kSplitMinTiles = 2;
-constexpr size_t kTicketBytes = 8192;   // [2 x SMs]
+constexpr size_t kTicketBytes = 8192;   // the split kernel's [2 x SMs], then the prompt kernel's [SMs]
 
 template <typename T, int D, int WM>
 size_t split_ws_floats(int sm_count)
@@ -792,7 +792,8 @@ size_t attend_ws_bytes(int sm_count)
                         split_ws_floats<__half, 128, 4>(sm_count), split_ws_floats<__half, 256, 4>(sm_count)};
     size_t most = 0;
     for (size_t x : f) most = x > most ? x : most;
-    return kTicketBytes + most * sizeof(float);
+    const size_t split = most * sizeof(float), prompt = attend_prompt_ws_bytes(sm_count);
+    return kTicketBytes + (split > prompt ? split : prompt);
 }
 size_t attend_ticket_bytes() { return kTicketBytes; }
 
@@ -800,7 +801,7 @@ int32_t launch_attend(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s
                       const GemvTuning& tune, int* launches)
 {
     *launches = 1;
-    if (attend_prompt_eligible(c, s, a)) return launch_attend_prompt(st, c, s, r, a, tune);
+    if (attend_prompt_eligible(c, s, a)) return launch_attend_prompt(st, c, s, r, a, ws, kTicketBytes, tune);
     switch (c.dim) {
     case 64: return c.bf16 ? launch_attend_td<__nv_bfloat16, 64>(st, c, s, r, a, ws, tune) : launch_attend_td<__half, 64>(st, c, s, r, a, ws, tune);
     case 128: return c.bf16 ? launch_attend_td<__nv_bfloat16, 128>(st, c, s, r, a, ws, tune) : launch_attend_td<__half, 128>(st, c, s, r, a, ws, tune);

@@ -49,6 +49,7 @@ struct PromptCfg {
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static constexpr int kSmem = kFixed + kStages * kStageBytes;
     static constexpr int kOCol = 2 * kKeys;                // tensor memory: S0 | S1 | O (one per row tile)
+    static constexpr int kPieceFloats = kRows * (D + 2);   // of a block whose keys several CTAs share: [D / 4][row][4], then m, l
     static_assert(kStages >= 3 && kOCol + kTilesQ * D <= 512, "shared and tensor memory");
 };
 constexpr float kSlack = 6.0f;         // log2 units
@@ -58,8 +59,18 @@ struct PromptBars {
     uint64_t full[8], empty[8];
     uint64_t s_full[2], p_full[2], pv_done[2], turn[2];
     uint32_t tmem;
-    int tainted;
+    int tainted, last;
 };
+// Few blocks against many keys (a chunk of a prompt on a long cache) would leave most SMs idle: `splits` CTAs then share a
+// block's keys, each leaving a piece, and the last one joins them in order.
+struct PromptWork {
+    float* pieces;       // [block][split][piece]
+    unsigned* tickets;   // [block], zero between launches
+    int* status;
+    int splits;
+};
+constexpr int kPromptMinTiles = 4;     // per CTA: less is lost in its set-up
+constexpr int kPromptMaxSplits = 8;
 
 // B operand whose rows are the summation index (V as it lies, [key][64 elements] swizzled rows): 8-row groups 1024 bytes
 // apart, runs of 64 elements `run` bytes apart.
@@ -201,7 +212,7 @@ __device__ __forceinline__ void regs_fewer()
 template <typename T, int D>
 __global__ void __launch_bounds__(PromptCfg<T, D>::kThreads, 1)
 attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, KvCacheView c, KvSeqsView s,
-                     RopeView rope, AttendArgs a, int* status)
+                     RopeView rope, AttendArgs a, PromptWork wk)
 {
     using C = PromptCfg<T, D>;
     constexpr bool BF = C::kBf16;
@@ -230,7 +241,11 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     }
     if (seq == s.seqs) return;
     const AttendBlock b = attend_block(c, s, span, group, C::kRows, a.window, nb - 1 - blk);
-    const int t0 = b.lo / KT, tiles = kv_max(1, (b.hi + KT - 1) / KT - t0);
+    const int first_tile = b.lo / KT, all_tiles = kv_max(1, (b.hi + KT - 1) / KT - first_tile);
+    const int parts = kv_max(1, kv_min(wk.splits, all_tiles / kPromptMinTiles)), part = (int)blockIdx.y;
+    if (part >= parts) return;
+    const int t0 = first_tile + all_tiles * part / parts, tiles = first_tile + all_tiles * (part + 1) / parts - t0;
+    float4* piece = reinterpret_cast<float4*>(wk.pieces + ((size_t)blockIdx.x * wk.splits + part) * C::kPieceFloats);
 
     if (warp == C::kSoftWarps) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem)), "r"(512) : "memory");
@@ -323,7 +338,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     auto wait = [&](uint64_t* which, uint32_t parity, int code) {
         if (dead || mbar_wait(which, parity)) return;
         dead = true;
-        if (status) atomicExch(status, code);
+        if (wk.status) atomicExch(wk.status, code);
     };
     // keys every row of the block sees: tiles inside need no mask
     const int lo_all = kv_seen_lo(span.pos(b.j1), a.window), hi_all = kv_seen_hi(c, s, span.pos(b.j0));
@@ -545,14 +560,20 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
         wait(&bar->pv_done[x], (tiles - 1) & 1, 57);
         tc_fence_after();
-        const float inv = m == -INFINITY || l == 0.0f ? 0.0f : 1.0f / l;   // no key seen: zeros, whatever the polynomials' 2^-126 sum to
+        if (m == -INFINITY) l = 0.0f;   // no key seen, whatever the polynomials' 2^-126 sum to
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + j_tok) * a.ldo + (size_t)(head * group + r % group) * D;
 #pragma unroll 1
         for (int i = 0; i < D / 32; i++) {
             uint32_t v[32];
             tmem_ld32_nowait(tmem + lanes + C::kOCol + x * D + 32 * i, v);
             tmem_wait_ld(v);
-            if (have) {
+            if (parts > 1) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    piece[(size_t)(8 * i + e) * C::kRows + row] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
+                                                                             __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
+            } else if (have) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     uint32_t y[4];
@@ -563,6 +584,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 }
             }
         }
+        if (parts > 1) reinterpret_cast<float2*>(piece + (size_t)(D / 4) * C::kRows)[row] = make_float2(m, l);
         tc_fence_before();
         if constexpr (C::kTrade) {
             named_bar_sync(2 + x, 128);
@@ -582,18 +604,74 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             for (int e = lane; e < D; e += 32) q[e] = rope_element(rope, src, e, pos) * (a.scale * kLog2e);
             __syncwarp();
             float m, l, acc[D / 32];
-            attend_row_plain<T, D>(c, s, seq, head, q, kv_seen_lo(pos, a.window), kv_seen_hi(c, s, pos), lane, &m, &l, acc);
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + j) * a.ldo + (size_t)h * D;
+            attend_row_plain<T, D>(c, s, seq, head, q, kv_max(kv_seen_lo(pos, a.window), t0 * KT), kv_min(kv_seen_hi(c, s, pos), (t0 + tiles) * KT), lane,
+                                   &m, &l, acc);
+            if (parts > 1) {
 #pragma unroll
-            for (int e = 0; e < D / 32; e++) out[lane + 32 * e] = __float2bfloat16_rn(acc[e] * inv);
+                for (int e = 0; e < D / 32; e++) {
+                    const int at = lane + 32 * e;
+                    reinterpret_cast<float*>(piece + (size_t)(at / 4) * C::kRows + row)[at & 3] = acc[e];
+                }
+                if (lane == 0) reinterpret_cast<float2*>(piece + (size_t)(D / 4) * C::kRows)[row] = make_float2(m, l);
+            } else {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + j) * a.ldo + (size_t)h * D;
+#pragma unroll
+                for (int e = 0; e < D / 32; e++) out[lane + 32 * e] = __float2bfloat16_rn(acc[e] * inv);
+            }
         }
+    }
+    if (parts == 1) return;
+    // ---- the join, by the CTA that finishes last: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i, thread = row
+    __syncthreads();
+    if (tid == 0) {
+        unsigned before;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(wk.tickets + blockIdx.x) : "memory");
+        bar->last = before == (unsigned)(parts - 1);
+        if (bar->last) wk.tickets[blockIdx.x] = 0;
+    }
+    __syncthreads();
+    if (!bar->last || tid >= b.rows) return;
+    const float4* p0 = reinterpret_cast<const float4*>(wk.pieces + (size_t)blockIdx.x * wk.splits * C::kPieceFloats) + tid;
+    float f[kPromptMaxSplits], mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPromptMaxSplits; i++) {
+        const float2 ml = i < parts ? __ldcg(reinterpret_cast<const float2*>(p0 - tid + (size_t)i * (C::kPieceFloats / 4) + (size_t)(D / 4) * C::kRows) + tid)
+                                    : make_float2(-INFINITY, 0.0f);
+        f[i] = ml.x;
+        mx = fmaxf(mx, ml.x);
+    }
+    const float base = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+    for (int i = 0; i < kPromptMaxSplits; i++) {
+        f[i] = ex2_approx(f[i] - base);
+        if (i < parts)
+            sum = fmaf(__ldcg(reinterpret_cast<const float2*>(p0 - tid + (size_t)i * (C::kPieceFloats / 4) + (size_t)(D / 4) * C::kRows) + tid).y, f[i], sum);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int r = b.r0 + tid;
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + r / group) * a.ldo + (size_t)(head * group + r % group) * D;
+#pragma unroll 2
+    for (int e = 0; e < D / 4; e++) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kPromptMaxSplits; i++) {
+            if (i < parts) {
+                const float4 v = __ldcg(p0 + (size_t)i * (C::kPieceFloats / 4) + (size_t)e * C::kRows);
+                acc.x = fmaf(v.x, f[i], acc.x);
+                acc.y = fmaf(v.y, f[i], acc.y);
+                acc.z = fmaf(v.z, f[i], acc.z);
+                acc.w = fmaf(v.w, f[i], acc.w);
+            }
+        }
+        *reinterpret_cast<uint2*>(out + 4 * e) = make_uint2(pack2<true>(acc.x * inv, acc.y * inv), pack2<true>(acc.z * inv, acc.w * inv));
     }
 }
 
 namespace {
 template <typename T, int D>
-int32_t launch_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a, const GemvTuning& tune)
+int32_t launch_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a, void* ws, size_t ticket_bytes,
+                      const GemvTuning& tune)
 {
     using C = PromptCfg<T, D>;
     static bool attr_done[64] = {};
@@ -612,26 +690,39 @@ int32_t launch_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s
         set_last_error("%d tokens x %d heads is more than one launch covers", s.tokens, a.heads);
         return kErrShape;
     }
-    FERRIC_CUDA_TRY(launch_kernel(attend_prompt_kernel<T, D>, dim3((unsigned)(blocks * c.heads)), dim3(C::kThreads), C::kSmem, st, tune.pdl, kmap, vmap,
-                                  c, s, r, a, gemm_status_word()));
+    // a block's keys are shared only as far as its CTAs then fit the device at once (one per SM)
+    PromptWork wk;
+    wk.splits = (int)(tune.sm_count / (blocks * c.heads));
+    wk.splits = wk.splits < 1 ? 1 : (wk.splits > kPromptMaxSplits ? kPromptMaxSplits : wk.splits);
+    wk.tickets = reinterpret_cast<unsigned*>(reinterpret_cast<uint8_t*>(ws) + ticket_bytes / 2);   // (the first half is the split kernel's)
+    wk.pieces = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + ticket_bytes);
+    wk.status = gemm_status_word();
+    FERRIC_CUDA_TRY(launch_kernel(attend_prompt_kernel<T, D>, dim3((unsigned)(blocks * c.heads), (unsigned)wk.splits), dim3(C::kThreads), C::kSmem, st, tune.pdl,
+                                  kmap, vmap, c, s, r, a, wk));
     return kOk;
 }
 }  // namespace
 
-// Prompts pay for tiles of 256 query rows (one sequence's tokens x query heads per key-value head) and whole CTAs per block;
-// below that, and where a result is wanted in f32, the split kernel runs.
+// Above 32 query rows a sequence and key-value head the tensor cores' tiles of 128 rows win although most of one is empty
+// (8 sequences x 2000 keys, 40 over 8 heads x 128 in bf16: 35 rows 57 us against the split kernel's 86; 65 rows 56 against
+// 138); where a result is wanted in f32, the split kernel runs.
 bool attend_prompt_eligible(const KvCacheView& c, const KvSeqsView& s, const AttendArgs& a)
 {
-    if (!a.out_bf16) return false;
-    const long long rows = (long long)s.tokens / s.seqs * (a.heads / c.heads);
-    return rows >= 128;
+    return a.out_bf16 && ((long long)s.tokens + s.seqs - 1) / s.seqs * (a.heads / c.heads) > 32;
 }
-int32_t launch_attend_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a, const GemvTuning& tune)
+size_t attend_prompt_ws_bytes(int sm_count)
+{
+    const size_t most = PromptCfg<__half, 256>::kPieceFloats > PromptCfg<__half, 128>::kPieceFloats ? PromptCfg<__half, 256>::kPieceFloats
+                                                                                                  : PromptCfg<__half, 128>::kPieceFloats;
+    return (size_t)sm_count * most * sizeof(float);
+}
+int32_t launch_attend_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s, const RopeView& r, const AttendArgs& a, void* ws, size_t ticket_bytes,
+                             const GemvTuning& tune)
 {
     switch (c.dim) {
-    case 64: return c.bf16 ? launch_prompt<__nv_bfloat16, 64>(st, c, s, r, a, tune) : launch_prompt<__half, 64>(st, c, s, r, a, tune);
-    case 128: return c.bf16 ? launch_prompt<__nv_bfloat16, 128>(st, c, s, r, a, tune) : launch_prompt<__half, 128>(st, c, s, r, a, tune);
-    default: return c.bf16 ? launch_prompt<__nv_bfloat16, 256>(st, c, s, r, a, tune) : launch_prompt<__half, 256>(st, c, s, r, a, tune);
+    case 64: return c.bf16 ? launch_prompt<__nv_bfloat16, 64>(st, c, s, r, a, ws, ticket_bytes, tune) : launch_prompt<__half, 64>(st, c, s, r, a, ws, ticket_bytes, tune);
+    case 128: return c.bf16 ? launch_prompt<__nv_bfloat16, 128>(st, c, s, r, a, ws, ticket_bytes, tune) : launch_prompt<__half, 128>(st, c, s, r, a, ws, ticket_bytes, tune);
+    default: return c.bf16 ? launch_prompt<__nv_bfloat16, 256>(st, c, s, r, a, ws, ticket_bytes, tune) : launch_prompt<__half, 256>(st, c, s, r, a, ws, ticket_bytes, tune);
     }
 }
 

@@ -235,6 +235,27 @@ def test_prompts(F, ctx, out_dtype, dtype, dim):
     b.check_attend(out_dtype=out_dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 1), (128, 5, 1), (256, 2, 2)])
+@pytest.mark.parametrize("window", [0, 900])
+def test_chunk_on_a_long_cache(F, ctx, dtype, dim, heads, kv_heads, window):
+    """Few blocks against many keys: several CTAs share a block's keys."""
+    b = Batch(F, ctx, lens=[2600, 1], new=[57, 1], heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype, page=32, base=1e6)
+    y = b.check_attend(out_dtype=BF, window=window)
+    assert torch.equal(b.check_attend(out_dtype=BF, window=window), y)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_chunk_on_a_long_cache_with_what_is_not_finite(F, ctx, bad):
+    b = Batch(F, ctx, lens=[2600], new=[57], heads=5, kv_heads=1, page=32)
+    want, bound, _ = R.attend(b.cache.k, b.cache.v, b.table, b.lens, b.starts, b.q, 5, b.rope_ref, out_dtype=BF)
+    b.cache.v[int(b.table[0, 2590 // 32]), 0, 2590 % 32, 7] = bad
+    y = b.cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=BF).double().cpu()
+    sees = torch.arange(2543, 2600) >= 2590
+    assert ((y - want).abs() <= bound)[~sees].all()
+    assert not torch.isfinite(y.reshape(57, 5, 128)[sees][:, :, 7]).any()
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_prompt_pages(F, ctx, page, dtype):
