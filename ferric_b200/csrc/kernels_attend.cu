@@ -413,8 +413,8 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     mma_kv<BF>(sc[2 * np], A[0], A[1], A[2], A[3], kf[0], kf[1]);
                     mma_kv<BF>(sc[2 * np + 1], A[0], A[1], A[2], A[3], kf[2], kf[3]);
                     if constexpr (BF) {
-                        mma_kv<BF>(sc[2 * np], E[0], 0u, E[1], 0u, kf[0], kf[1]);
-                        mma_kv<BF>(sc[2 * np + 1], E[0], 0u, E[1], 0u, kf[2], kf[3]);
+                        mma_kv<BF>(sc[2 * np], 0u, E[0], 0u, E[1], kf[0], kf[1]);
+                        mma_kv<BF>(sc[2 * np + 1], 0u, E[0], 0u, E[1], kf[2], kf[3]);
                     }
                 }
             }
@@ -480,8 +480,8 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     mma_kv<BF>(o[2 * np], P[0], P[1], P[2], P[3], vf[0], vf[1]);
                     mma_kv<BF>(o[2 * np + 1], P[0], P[1], P[2], P[3], vf[2], vf[3]);
                     if constexpr (BF) {
-                        mma_kv<BF>(o[2 * np], E[0], 0u, E[1], 0u, vf[0], vf[1]);
-                        mma_kv<BF>(o[2 * np + 1], E[0], 0u, E[1], 0u, vf[2], vf[3]);
+                        mma_kv<BF>(o[2 * np], 0u, E[0], 0u, E[1], vf[0], vf[1]);
+                        mma_kv<BF>(o[2 * np + 1], 0u, E[0], 0u, E[1], vf[2], vf[3]);
                     }
                 }
                 if (MASKED && odd && b.j0 != b.j1) bar->tainted = 1;
