@@ -167,37 +167,6 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b)
     return r;
 }
 
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-// 2^x for a pair, x at most 127: x = n + f with n the nearest whole number (adding 1.5 * 2^23 leaves it in the low bits) and
-// |f| <= 1/2, 2^f by the polynomial of degree 4 whose largest relative error there is least (Remez exchange in 64 bits;
-// 2.7e-6 evaluated in floats, a 700th of what the weights are rounded to in bf16 and a 90th in f16), times 2^n.  Below
-// 2^-126 the weight is 2^-126.  A NaN stays one.
-__device__ __forceinline__ void ex2_poly2(uint64_t x, float& p0, float& p1)
-{
-    float a, b;
-    unpack_f32x2(x, a, b);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.0f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.0f));
-    x = pack_f32x2(a, b);
-    const uint64_t magic = pack_f32x2(12582912.0f, 12582912.0f), minus_magic = pack_f32x2(-12582912.0f, -12582912.0f);
-    const uint64_t t = add_f32x2(x, magic), n = add_f32x2(t, minus_magic);
-    const uint64_t f = fma_f32x2(n, pack_f32x2(-1.0f, -1.0f), x);
-    uint64_t y = fma_f32x2(f, pack_f32x2(0.00957010191f, 0.00957010191f), pack_f32x2(0.0559178603f, 0.0559178603f));
-    y = fma_f32x2(y, f, pack_f32x2(0.240247448f, 0.240247448f));
-    y = fma_f32x2(y, f, pack_f32x2(0.693121815f, 0.693121815f));
-    y = fma_f32x2(y, f, pack_f32x2(0.999999261f, 0.999999261f));
-    float ta, tb, ya, yb;
-    unpack_f32x2(t, ta, tb);
-    unpack_f32x2(y, ya, yb);
-    // low bits of t: n; 2^n as a float has n + 127 in its exponent field
-    p0 = ya * __int_as_float(__float_as_int(ta) * (1 << 23) + 0x3f800000);
-    p1 = yb * __int_as_float(__float_as_int(tb) * (1 << 23) + 0x3f800000);
-}
 template <int N>
 __device__ __forceinline__ void regs_more()
 {
@@ -531,19 +500,13 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const float base = m == -INFINITY ? 0.0f : m;
             const uint64_t minus = pack_f32x2(-base, -base);
             uint64_t sum[2] = {0, 0};
-            // A quarter of the exponentials run as polynomials on the FMA pipe: ex2 retires 4 lanes a cycle and scheduler, and 128
-            // a row and tile would be the loop's bound.
 #pragma unroll
             for (int i = 0; i < KT / 2; i++) {
                 const uint64_t x = add_f32x2(pack_f32x2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])), minus);
                 float p0, p1;
-                if (i % 4 == 3) {
-                    ex2_poly2(x, p0, p1);
-                } else {
-                    unpack_f32x2(x, p0, p1);
-                    p0 = ex2_approx(p0);
-                    p1 = ex2_approx(p1);
-                }
+                unpack_f32x2(x, p0, p1);
+                p0 = ex2_approx(p0);
+                p1 = ex2_approx(p1);
                 sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(p0, p1));
                 w[i] = pack2<BF>(p0, p1);
                 if (i % 16 == 15) tmem_st16(s_col + (i - 15), w + (i - 15));
@@ -560,7 +523,6 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
         wait(&bar->pv_done[x], (tiles - 1) & 1, 57);
         tc_fence_after();
-        if (m == -INFINITY) l = 0.0f;   // no key seen, whatever the polynomials' 2^-126 sum to
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + j_tok) * a.ldo + (size_t)(head * group + r % group) * D;
 #pragma unroll 1
