@@ -199,16 +199,27 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 
     // ---- this CTA's block: the heads' blocks side by side, each sequence's longest first, so that short ones fill up the end
     const int head = (int)(blockIdx.x % (unsigned)c.heads);
-    int seq = 0, blk = (int)(blockIdx.x / (unsigned)c.heads);
-    KvSpan span{};
-    int nb = 0;
-    for (; seq < s.seqs; seq++) {
-        span = kv_span(s, seq);
-        nb = attend_blocks(span, group, C::kRows);
-        if (blk < nb) break;
-        blk -= nb;
+    int seq = -1, blk = (int)(blockIdx.x / (unsigned)c.heads);
+    for (int i0 = 0; i0 < s.seqs; i0 += 32) {   // 32 sequences at a time, every warp for itself
+        const int mine = i0 + lane < s.seqs ? attend_blocks(kv_span(s, i0 + lane), group, C::kRows) : 0;
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, blk < incl);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            seq = i0 + at;
+            blk -= __shfl_sync(0xffffffffu, incl - mine, at);
+            break;
+        }
+        blk -= __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (seq == s.seqs) return;
+    if (seq < 0) return;
+    const KvSpan span = kv_span(s, seq);
+    const int nb = attend_blocks(span, group, C::kRows);
     const AttendBlock b = attend_block(c, s, span, group, C::kRows, a.window, nb - 1 - blk);
     const int first_tile = b.lo / KT, all_tiles = kv_max(1, (b.hi + KT - 1) / KT - first_tile);
     const int parts = kv_max(1, kv_min(wk.splits, all_tiles / kPromptMinTiles)), part = (int)blockIdx.y;

@@ -151,6 +151,18 @@ int32_t check_rows(const char* what, const float* p, size_t n, size_t cols, size
     return kOk;
 }
 
+// Whether n rows of `a_bytes` every `a_pitch` share memory with n rows of `b_bytes` every `b_pitch` (columns of one wider matrix
+// do not; other interleavings count as sharing).
+bool rows_overlap(const void* a, size_t a_pitch, size_t a_bytes, const void* b, size_t b_pitch, size_t b_bytes, size_t n)
+{
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), a1 = a0 + (n - 1) * a_pitch + a_bytes;
+    const uintptr_t b0 = reinterpret_cast<uintptr_t>(b), b1 = b0 + (n - 1) * b_pitch + b_bytes;
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (a_pitch != b_pitch) return true;
+    const uintptr_t d = b0 >= a0 ? (b0 - a0) % a_pitch : (a_pitch - (a0 - b0) % a_pitch) % a_pitch;   // b's columns from a's first
+    return d < a_bytes || d + b_bytes > a_pitch;
+}
+
 }  // namespace
 
 extern "C" {
@@ -284,6 +296,10 @@ int32_t ferric_cuda_kv_attend(ferric_cuda_ctx* ctx, const ferric_kv_cache* cache
     }
     if (misaligned(out_dev, 16)) {
         set_last_error("the result must be 16-byte aligned");
+        return kErrInvalidArg;
+    }
+    if (n_tokens > 0 && rows_overlap(q_dev, ldq * 4, cols * 4, out_dev, ldo * out_size, cols * out_size, n_tokens)) {
+        set_last_error("the result overlaps q, which other rows still need");
         return kErrInvalidArg;
     }
     if (!isfinite(scale)) {

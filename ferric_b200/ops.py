@@ -113,6 +113,10 @@ class Context:
     def reserve_scratch(self, nbytes: int) -> None:
         _check(self._lib.ferric_cuda_ctx_reserve_scratch(self._h, nbytes), "reserve_scratch")
 
+    def attend_reserve(self) -> None:
+        """Allocate the attention's workspace now (``ferric_cuda_attend_reserve``), before a capture that attends."""
+        _check(self._lib.ferric_cuda_attend_reserve(self._h), "attend_reserve")
+
     def chain_reserve(self, slot_bytes: int) -> None:
         """Size the two prepared-activation slots chained products use (``ferric_cuda_chain_reserve``)."""
         _check(self._lib.ferric_cuda_chain_reserve(self._h, slot_bytes), "chain_reserve")

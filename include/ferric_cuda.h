@@ -375,7 +375,7 @@ int32_t ferric_cuda_kv_append(ferric_cuda_ctx *ctx, const ferric_kv_cache *cache
  * h / (n_q_heads / cache heads).  q is f32 like k above (rotated here: `rope` as for append); scale 0 = 1 / sqrt(head_dim).
  * out is FERRIC_GGML_F32 (the decode products' activation type: the whole product is then kept to f32 accuracy) or
  * FERRIC_GGML_BF16 (the prefill products'), 16-byte aligned with row stride ldo (0 = dense; a multiple of 16 bytes), and
- * must not overlap q.  A token that sees no key gets zeros; output rows outside every sequence are left as they were.  The
+ * must not overlap q (refused).  A token that sees no key gets zeros; output rows outside every sequence are left as they were.  The
  * new tokens' own keys must have been appended.  A key or value element that is not finite reaches only the tokens that see it.
  * Calls on one context share a workspace (ferric_cuda_attend_reserve, allocated by the first call otherwise, which must then
  * not be under capture): graphs captured on one context must not be replayed at the same time -- give each stream of

@@ -396,6 +396,54 @@ def test_captured_step_follows_lengths_and_pages(F, ctx):
     assert b.seqs.lens.tolist() == b.lens
 
 
+def test_capture_before_anything_has_run(F):
+    """Without a workspace a capture is refused, and stays usable; with it reserved the first call may be captured."""
+    c = F.Context(0)
+    b = Batch(F, c, lens=[300, 5], heads=8, kv_heads=2, page=16)
+    out = torch.zeros((2, 8 * 128), device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        c.use_torch_stream()
+        with pytest.raises(F.FerricError) as e:
+            b.cache.attend(b.seqs, b.q, rope=b.rope, out=out)
+        out.add_(1.0)
+    assert "attend_reserve" in str(e.value)
+    g.replay()
+    torch.cuda.synchronize()
+    assert (out == 1.0).all()
+    c.use_torch_stream()
+    c.attend_reserve()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        c.use_torch_stream()
+        b.cache.attend(b.seqs, b.q, rope=b.rope, out=out)
+    g.replay()
+    torch.cuda.synchronize()
+    c.use_torch_stream()
+    assert torch.equal(out, b.check_attend())
+    c.close()
+
+
+def test_result_on_top_of_q_is_refused(F, ctx):
+    b = Batch(F, ctx, lens=[100, 5], heads=8, kv_heads=2, page=16)
+    with pytest.raises(F.FerricError):
+        b.cache.attend(b.seqs, b.q, rope=b.rope, out=b.q)
+    want = b.cache.attend(b.seqs, b.q, rope=b.rope)
+    wide = torch.zeros((2, 2 * 8 * 128), device="cuda")          # columns beside q's are fine
+    wide[:, :1024] = b.q
+    b.cache.attend(b.seqs, wide[:, :1024], rope=b.rope, out=wide[:, 1024:])
+    assert torch.equal(wide[:, 1024:], want) and torch.equal(wide[:, :1024], b.q)
+
+
+def test_prompts_of_many_sequences(F, ctx):
+    """More sequences than one warp looks over at a time, some without new tokens."""
+    new = [(7 * i) % 23 for i in range(101)]
+    b = Batch(F, ctx, lens=[n + i % 40 for i, n in enumerate(new)], new=new, heads=4, kv_heads=1, dim=64, page=16)
+    b.check_attend(out_dtype=BF)
+
+
 def test_two_contexts_on_two_streams(F):
     """Graphs of two contexts replayed at the same time: each has a workspace of its own."""
     runs = []

@@ -159,7 +159,7 @@ def call(lib, fn, c=None, s=None, n=3, **kw):
         d.update(kw)
         rc = lib.ferric_cuda_kv_append(None, cp, sp, None, d["k"], d["ldk"], d["v"], d["ldv"], n)
     else:
-        d = dict(q=P, ldq=0, heads=8, scale=0.0, window=0, out=P, ty=0, ldo=0)
+        d = dict(q=P, ldq=0, heads=8, scale=0.0, window=0, out=4 * P, ty=0, ldo=0)
         d.update(kw)
         rc = lib.ferric_cuda_kv_attend(None, cp, sp, None, d["q"], d["ldq"], n, d["heads"], d["scale"], d["window"], d["out"], d["ty"], d["ldo"])
     return rc, lib.ferric_cuda_last_error().decode()
@@ -200,6 +200,14 @@ def test_bad_operands(lib):
                    (dict(heads=3), 3), (dict(heads=0), 3), (dict(ty=1), 2), (dict(ty=30, ldo=1028), 3), (dict(scale=float("nan")), 1),
                    (dict(scale=float("inf")), 1), (dict(heads=1 << 20), 3)]:
         assert call(lib, "attend", **kw)[0] == rc, kw
+    # a result on top of q is refused, one in other columns of the same rows is not
+    for kw in [dict(q=P, out=P), dict(q=P, out=P + 16), dict(q=P + 4096, out=P), dict(q=P, ldq=4096, out=P + 4080, ldo=4096),
+               dict(q=P, ldq=4096, out=P + 16384 * 2 - 16, ldo=4096), dict(q=P, ldq=4096, out=P + 4096, ldo=2048), dict(q=P, out=P + 4096, ty=30)]:
+        got = call(lib, "attend", **{"out": P, **kw})
+        assert got[0] == 1 and "overlaps" in got[1], kw
+    for kw in [dict(q=P, ldq=4096, out=P + 4096, ldo=4096), dict(q=P + 4096, ldq=4096, out=P, ldo=4096), dict(q=P, out=P + 3 * 4096),
+               dict(q=P + 3 * 4096, out=P)]:
+        assert call(lib, "attend", **kw)[1] == "NULL context", kw
     assert call(lib, "attend", ty=30, ldo=1032)[1] == "NULL context"
     h = C.c_void_p()
     assert lib.ferric_cuda_rope_create(None, 64, 1e4, None, 0, C.byref(h)) == 1
