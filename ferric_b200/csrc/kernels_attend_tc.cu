@@ -535,7 +535,9 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         wait(&bar->pv_done[x], (tiles - 1) & 1, 57);
         tc_fence_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + j_tok) * a.ldo + (size_t)(head * group + r % group) * D;
+        // The result goes through the tile's place of Q, done with since its last S: written row by row as tensor memory
+        // holds it (16-byte chunks, permuted so that eight rows do not meet in a bank), stored row-contiguously.
+        uint8_t* stage = qs + x * (C::kParts * 128 * D * 2) + (warp & 3) * 32 * (D * 2);
 #pragma unroll 1
         for (int i = 0; i < D / 32; i++) {
             uint32_t v[32];
@@ -546,15 +548,29 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 for (int e = 0; e < 8; e++)
                     piece[(size_t)(8 * i + e) * C::kRows + row] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
                                                                              __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
-            } else if (have) {
+            } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     uint32_t y[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++)
                         y[k] = pack2<true>(__uint_as_float(v[8 * e + 2 * k]) * inv, __uint_as_float(v[8 * e + 2 * k + 1]) * inv);
-                    *reinterpret_cast<uint4*>(out + 32 * i + 8 * e) = make_uint4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint4*>(stage + lane * (D * 2) + (((4 * i + e) ^ (lane & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
+            }
+        }
+        if (parts == 1) {
+            __syncwarp();
+            unsigned long long mine = 0;      // where this lane's row goes
+            if (have)
+                mine = reinterpret_cast<unsigned long long>(reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first + j_tok) * a.ldo +
+                                                            (size_t)(head * group + r % group) * D);
+            constexpr int kLanes = D / 8;     // of a row
+#pragma unroll 4
+            for (int i = 0; i < kLanes; i++) {
+                const int rr = i * (32 / kLanes) + lane / kLanes, ch = lane % kLanes;
+                const unsigned long long to = __shfl_sync(0xffffffffu, mine, rr);
+                if (to) *reinterpret_cast<uint4*>(to + 16 * ch) = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((ch ^ (rr & 7)) << 4));
             }
         }
         if (parts > 1) reinterpret_cast<float2*>(piece + (size_t)(D / 4) * C::kRows)[row] = make_float2(m, l);
