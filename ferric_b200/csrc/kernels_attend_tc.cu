@@ -532,6 +532,9 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->p_full[sb]);
         }
+        // A parity only tells neighbouring phases apart.  Where S runs two units ahead, the last S says that the products up to
+        // unit tiles - 3 are done, so the one before the last is waited for too.
+        if (PRE == 2 && tiles > 1) wait(&bar->pv_done[x], (tiles - 2) & 1, 57);
         wait(&bar->pv_done[x], (tiles - 1) & 1, 57);
         tc_fence_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;

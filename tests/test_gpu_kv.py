@@ -73,6 +73,17 @@ class Batch:
         self.rope = F.Rope(ctx, rotary, base=base, interleaved=interleaved) if rotary else None
         self.rope_ref = dict(rotary=rotary, base=base, interleaved=interleaved) if rotary else dict(rotary=0)
 
+    def check_rows(self, got, want, mine, out_dtype):
+        """Row by row: the bound above adds up what roundings of q and of the weights could do together, which for a bf16 result
+        over many keys is more than the result.  They are independent: result, weights and q are each off by at most 2^-8 of
+        their terms, 2^-8 / sqrt(3) in the mean square, together at most 2^-8 of the row's length for values around 0; twice
+        that is the limit here.  An f32 result has its derived bound."""
+        if out_dtype != BF:
+            return
+        d = (got - want)[mine].reshape(-1, self.dim).norm(dim=1)
+        n = want[mine].reshape(-1, self.dim).norm(dim=1)
+        assert (d <= 2.0 ** -7 * n + 1e-12).all(), f"a row is {float((d / n.clamp(min=1e-12)).max()):.3g} off"
+
     def check_attend(self, window=0, out_dtype=torch.float32, scale=None):
         mark = torch.full((self.tokens, self.heads * self.dim), 7.0, dtype=out_dtype, device="cuda")
         y = self.cache.attend(self.seqs, self.q, rope=self.rope, window=window, scale=scale, out=mark)
@@ -84,6 +95,7 @@ class Batch:
         off = (got - want)[mine].abs()
         assert torch.isfinite(got[mine]).all()
         assert (off <= bound[mine]).all(), f"worst {float((off / bound[mine].clamp(min=1e-30)).max()):.3g} of the bound"
+        self.check_rows(got, want, mine, out_dtype)
         return y
 
 
