@@ -16,7 +16,8 @@ int* gemm_status_word();   // device address of the status word shared with the 
 // ---------------------------------------------------------------------------------------------------------------------
 // attend_split_kernel: few query rows against many keys, kept to f32 accuracy.
 //
-// Bound by the cache's bytes from HBM (2 * 2 * head_dim per key and head; at 5 query heads per key-value head that is 5
+// 64 sequences over 0.7k-8k keys (40 over 8 heads x 128, f16): 190 us = 6.2 TB/s; one over 131000 (bf16): 116-123 us = 4.4-4.6
+// TB/s, of which the stream itself takes about 80.  Bound by the cache's bytes from HBM (2 * 2 * head_dim per key and head; at 5 query heads per key-value head that is 5
 // multiply-adds per byte).  So: one CTA reads a tile of 64 keys once for all query heads of its key-value head, tiles travel
 // by TMA into a ring filled by a warp of its own, and the line of all tiles is cut evenly over the resident CTAs
 // (kv_index.h); a block that several CTAs share leaves pieces (m, l, unnormalised output) in the workspace, which the CTA
@@ -63,7 +64,8 @@ struct SplitWork {
     float* pieces;       // [CTA][2][piece]
     unsigned* tickets;   // [CTA], zero between launches
     int* status;
-    int min_tiles;       // tiles per CTA at least, while there are few
+    int min_tiles;       // tiles per CTA at least, while there are few ..
+    int min_parts;       // .. but as many CTAs as there are (sequence, head) pairs to do side by side
     unsigned long long group_recip;   // ceil(2^32 / group)
 };
 struct SplitBars {
@@ -198,7 +200,8 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         total += all;
     }
     if (total == 0) return;
-    const long long want = (total + wk.min_tiles - 1) / wk.min_tiles;
+    long long want = (total + wk.min_tiles - 1) / wk.min_tiles;
+    if (want < wk.min_parts) want = wk.min_parts < total ? wk.min_parts : total;
     const int parts = (int)(want < (long long)gridDim.x ? want : (long long)gridDim.x);
     if ((int)blockIdx.x >= parts) return;
     const long long x0 = attend_cut(total, parts, blockIdx.x), x1 = attend_cut(total, parts, blockIdx.x + 1);
@@ -737,6 +740,8 @@ int32_t encode_cache(CUtensorMap* map, const KvCacheView& c, void* base, const v
 }
 
 namespace {
+// Two tiles a CTA at least: joining a block of two tiles costs more than its second tile (1 x 100 keys, 40 over 8 heads:
+// 12.3 us on sixteen CTAs and eight joins, 8.4 us on eight).
 constexpr int kSplitMinTiles = 2;
 constexpr size_t kTicketBytes = 8192;   // the split kernel's [2 x SMs], then the prompt kernel's [SMs]
 
@@ -766,6 +771,7 @@ int32_t launch_split(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s,
     wk.pieces = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + kTicketBytes);
     wk.status = gemm_status_word();
     wk.min_tiles = kSplitMinTiles;
+    wk.min_parts = (int)((long long)s.seqs * c.heads < 4096 ? (long long)s.seqs * c.heads : 4096);
     wk.group_recip = (0x100000000ull + (unsigned)(a.heads / c.heads) - 1) / (unsigned)(a.heads / c.heads);
     FERRIC_CUDA_TRY(launch_kernel(attend_split_kernel<T, D, WM>, dim3((unsigned)(tune.sm_count * C::kMinCtas)), dim3(C::kThreads), C::kSmem, st,
                                   tune.pdl, kmap, vmap, c, s, r, a, wk));

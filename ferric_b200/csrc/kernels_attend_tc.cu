@@ -1,6 +1,8 @@
 // attend_prompt_kernel: attention of many new tokens (prompts and chunks of them), result in bf16, on tcgen05.
 //
-// Bound by the tensor cores (4 head_dim flop per visible pair and query head).  A CTA takes 256 query rows (head_dim 256:
+// A prompt of 4096 (40 over 8 heads x 128): 271 us = 635 TFLOP/s in bf16; chunks of three prompts in f16: 202 us = 937 TFLOP/s.
+// Bound by the tensor cores (4 head_dim flop per visible pair and query head), short of it by a block's set-up and end and, in
+// bf16, by a ring of three stages.  A CTA takes 256 query rows (head_dim 256:
 // 128) of one key-value head -- (token, query head of the group) pairs, so that all heads of the group share the keys it
 // reads -- and walks the keys they see in tiles.  Per tile and 128 rows, a "unit": S = Q K^T into tensor memory; one thread
 // per row takes the softmax step in registers and writes the weights back over S as 16-bit values; O += P V with P read
