@@ -280,6 +280,13 @@ def test_prompt_window(F, ctx, out_dtype, window):
     Batch(F, ctx, lens=[300, 90, 200], new=[290, 90, 140], heads=2, kv_heads=1, page=16).check_attend(window=window, out_dtype=out_dtype)
 
 
+@pytest.mark.parametrize("scale", [1.0, -1.0, 1e-4])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prompt_scales(F, ctx, dtype, scale):
+    """Scores over tens of log2 units, where the running maximum keeps moving, and scores that are all but equal."""
+    Batch(F, ctx, lens=[700], new=[140], heads=2, kv_heads=1, page=64, dtype=dtype).check_attend(out_dtype=BF, scale=scale)
+
+
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (40, 8), (12, 1), (64, 1), (129, 1), (200, 1)])
 def test_prompt_head_layouts(F, ctx, heads, kv_heads):
     Batch(F, ctx, lens=[70, 150], new=[70, 13], heads=heads, kv_heads=kv_heads, dim=64, page=64).check_attend(out_dtype=BF)
@@ -705,3 +712,10 @@ def test_refusals(F, ctx):
     with pytest.raises(ValueError):
         F.KVSeqs(b.seqs.page_table, b.seqs.lens[:1])
     b.check_attend()                                                              # and the context still works
+
+
+def test_no_wait_ran_out(F, ctx):
+    """Every wait in the kernels is bounded and leaves a code when it gives up: none of the calls above did."""
+    import ctypes as C
+    code = C.c_int32(-1)
+    assert ctx._lib.ferric_cuda_gemm_status(ctx._h, C.byref(code)) == 0 and code.value == 0
