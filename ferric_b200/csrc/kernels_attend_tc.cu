@@ -490,14 +490,21 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             for (int i = 0; i < KT; i += 2)
                 asm("max.f32 %0, %0, %1, %2;" : "+f"(mq[(i >> 1) & 3]) : "f"(__uint_as_float(w[i])), "f"(__uint_as_float(w[i + 1])));
             const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) - kShift;
+            // The products up to the unit before, complete.  A parity only tells neighbouring phases apart, so every phase is
+            // waited for once, in order, and before this unit's weights are handed over: its own products cannot have
+            // completed by then, and no later wait finds the barrier more than one phase away.
+            bool summed = j == 0;
+            auto wait_summed = [&] {
+                if (!summed) wait(&bar->pv_done[x], (j - 1) & 1, 56);
+                summed = true;
+            };
             const bool move = mx > m + kSlack || (m == -INFINITY && mx > m);
             if (__any_sync(0xffffffffu, move)) {
                 const float mn = move ? mx : m, fix = move ? ex2_approx(m - mn) : 1.0f;
                 m = mn;
                 l *= fix;
                 if (j > 0) {
-                    // O of the units before must be complete
-                    wait(&bar->pv_done[x], (j - 1) & 1, 56);
+                    wait_summed();
                     tc_fence_after();
 #pragma unroll 1
                     for (int i = 0; i < D / 32; i++) {
@@ -530,13 +537,11 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 l += a0 + a1;
             }
             tmem_wait_st();
+            wait_summed();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->p_full[sb]);
         }
-        // A parity only tells neighbouring phases apart.  Where S runs two units ahead, the last S says that the products up to
-        // unit tiles - 3 are done, so the one before the last is waited for too.
-        if (PRE == 2 && tiles > 1) wait(&bar->pv_done[x], (tiles - 2) & 1, 57);
         wait(&bar->pv_done[x], (tiles - 1) & 1, 57);
         tc_fence_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;

@@ -1,6 +1,7 @@
 """The paged key-value cache (append with rotation) and the attention over it against a 64-bit evaluation, through the
 framework's entry points, at the lengths, head layouts, pages and masks where such operators go wrong.  Tolerances are
 derived in ``kv_ref``."""
+import math
 import random
 
 import pytest
@@ -285,6 +286,25 @@ def test_prompt_window(F, ctx, out_dtype, window):
 def test_prompt_scales(F, ctx, dtype, scale):
     """Scores over tens of log2 units, where the running maximum keeps moving, and scores that are all but equal."""
     Batch(F, ctx, lens=[700], new=[140], heads=2, kv_heads=1, page=64, dtype=dtype).check_attend(out_dtype=BF, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens,new", [([900], [900]), ([1500, 333], [130, 70])])
+def test_prompt_scores_that_climb(F, ctx, dtype, dim, lens, new):
+    """The maximum moves in every key tile, by 7 log2 units.  Every other tile holds one key at its level and nothing else that
+    counts, so the tile before it, whole and 7 units lower, carries a third of the result: losing its products shows."""
+    b = Batch(F, ctx, lens=lens, new=new, heads=2, kv_heads=1, dim=dim, dtype=dtype, page=16, rotary=0)
+    b.q.mul_(0.1)
+    b.q[:, 0] = b.q[:, dim] = 1.0
+    tile = 64 if dim == 256 else 128
+    for i, n in enumerate(lens):
+        pos = torch.arange(n)
+        t = pos // tile
+        level = torch.where((t % 2 == 0) | (pos % tile == 0), 7.0 * t, 7.0 * t - 60.0).to(dtype).cuda()
+        pages = b.table[i][pos // 16].long().cuda()
+        b.cache.k[pages, 0, (pos % 16).cuda(), 0] = level
+    b.check_attend(out_dtype=BF, scale=math.log(2.0))
 
 
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (40, 8), (12, 1), (64, 1), (129, 1), (200, 1)])
