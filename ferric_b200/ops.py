@@ -496,9 +496,19 @@ class Rope:
             pass
 
 
+def _pitch(t: torch.Tensor, name: str) -> int:
+    """The stride between t[0], t[1], ... as the C ABI takes it.  It spells "dense" as 0, which is right for one row; torch's 0 for
+    several is one row in memory for all of them, and has no spelling there."""
+    if t.shape[0] <= 1:
+        return 0
+    if t.stride(0) == 0 and t.numel():
+        raise ValueError(f"{name} is an expanded tensor, one row in memory for all {t.shape[0]}: pass {name}.contiguous()")
+    return t.stride(0)
+
+
 class KVSeqs:
     """The batch a cache call works on (``ferric_kv_seqs``), int32 CUDA tensors read when the kernels run: ``page_table``
-    [n_seqs, max_pages]; ``lens`` [n_seqs], each sequence's length with its new tokens; ``starts`` [n_seqs + 1], the first
+    [n_seqs, max_pages], each sequence with a row of its own (rows may name the same pages); ``lens`` [n_seqs], each sequence's length with its new tokens; ``starts`` [n_seqs + 1], the first
     activation row of each sequence, or None when row i is the one new token of sequence i."""
 
     def __init__(self, page_table: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None):
@@ -513,7 +523,7 @@ class KVSeqs:
             raise ValueError("page_table, lens and starts must be on one device")
         self.page_table, self.lens, self.starts = page_table, lens, starts
         n, cols = page_table.shape
-        self._c = _lib.KvSeqs(page_table.data_ptr(), n, cols, page_table.stride(0) if n > 1 else 0, lens.data_ptr(),
+        self._c = _lib.KvSeqs(page_table.data_ptr(), n, cols, _pitch(page_table, "page_table"), lens.data_ptr(),
                               starts.data_ptr() if starts is not None else None)
         self._ref, self._dev = C.byref(self._c), lens.get_device()
 
@@ -539,7 +549,7 @@ class KVCache:
         self.ctx, self._lib, self.k, self.v = ctx, ctx._lib, k, v
         self.n_heads, self.page_size, self.head_dim = heads, page, dim
         self._c = _lib.KvCache(k.data_ptr(), v.data_ptr(), GGML_F16 if k.dtype == torch.float16 else GGML_BF16, n_pages, page, heads,
-                               dim, k.stride(0) if n_pages > 1 else 0)
+                               dim, _pitch(k, "k"))
         self._ref, self._dev = C.byref(self._c), ctx.device
 
     @classmethod
@@ -618,7 +628,7 @@ class KVCache:
         else:
             if out.shape != q.shape or out.device != q.device or (out.stride(1) != 1 and cols > 1):
                 raise TypeError("out must be a tensor of q's shape and device with adjacent columns")
-            ldo = out.stride(0) if n > 1 else 0
+            ldo = _pitch(out, "out")
         ty = GGML_F32 if out.dtype is torch.float32 else GGML_BF16
         if ty == GGML_BF16 and out.dtype is not torch.bfloat16:
             raise TypeError("the result is float32 or bfloat16")

@@ -541,6 +541,21 @@ def test_operands_that_are_not_dense(F, ctx):
     assert torch.equal(slot[:, 32:32 + b.heads * 128], want) and (slot[:, :32] == 5).all() and (slot[:, 32 + b.heads * 128:] == 5).all()
 
 
+def test_sequences_that_share_a_context(F, ctx):
+    """One row of pages for all: refused as an expanded tensor, right as a copy."""
+    b = Batch(F, ctx, lens=[90, 90, 90], heads=4, kv_heads=1, page=16)
+    row = b.table[1:2]
+    with pytest.raises(ValueError):
+        F.KVSeqs(row.cuda().expand(3, -1), b.seqs.lens)
+    with pytest.raises(ValueError):
+        b.cache.attend(b.seqs, b.q, out=torch.zeros(512, device="cuda").expand(3, 512))
+    with pytest.raises(ValueError):
+        F.KVCache(ctx, b.cache.k[:1].expand(4, -1, -1, -1), b.cache.v[:1].expand(4, -1, -1, -1))
+    b.table = row.expand(3, -1).contiguous()
+    b.seqs = F.KVSeqs(b.table.cuda(), b.seqs.lens)
+    b.check_attend()
+
+
 def test_no_tokens_and_no_sequences(F, ctx):
     b = Batch(F, ctx, lens=[20], new=[0])
     assert b.cache.attend(b.seqs, b.q, rope=b.rope).shape == (0, b.heads * b.dim)

@@ -216,6 +216,79 @@ def test_bad_operands(lib):
     assert call(lib, "append", c=False)[1] == "NULL cache" and call(lib, "attend", s=False)[1] == "NULL sequence table"
 
 
+# ---- what the Python layer hands to the C ABI -----------------------------------------------------------
+class Ctx:
+    """A context whose library records the calls, so that what Python passes on shows without a device."""
+
+    def __init__(self, device=0):
+        self.device, self._h, self._stream, self._lib, self.calls = device, P, 0, self, []
+
+    def __getattr__(self, name):
+        if not name.startswith("ferric_"):
+            raise AttributeError(name)
+        return lambda *a: self.calls.append((name, a)) or 0
+
+
+@pytest.fixture()
+def on_gpu(monkeypatch):
+    """Makes CPU tensors that say they are on cuda:0; calls go straight to the (recording) library."""
+    import torch
+
+    from ferric_b200 import ops
+
+    class OnGpu(torch.Tensor):
+        is_cuda = property(lambda self: True)
+        device = property(lambda self: torch.device("cuda", 0))
+
+        def get_device(self):
+            return 0
+
+    def run(self, fn, where, *args):
+        ops._check(fn(self.ctx._h, self._ref, *args), where)
+
+    monkeypatch.setattr(ops.KVCache, "_run", run)
+    return lambda t: t.as_subclass(OnGpu)
+
+
+def py_cache(on_gpu, ctx, n_pages=6, heads=2, page=16, dim=128):
+    import torch
+
+    from ferric_b200 import ops
+    z = lambda: on_gpu(torch.zeros((n_pages, heads, page, dim), dtype=torch.bfloat16))
+    return ops.KVCache(ctx, z(), z())
+
+
+def test_expanded_tensors_are_refused(on_gpu):
+    """A row stride of 0 means dense in the C ABI: passed on, an expanded tensor would be read or written behind its memory."""
+    import torch
+
+    from ferric_b200 import ops
+    i32 = lambda *s: on_gpu(torch.zeros(s, dtype=torch.int32))
+    with pytest.raises(ValueError, match="page_table.contiguous"):
+        ops.KVSeqs(i32(4).expand(3, 4), i32(3))
+    assert ops.KVSeqs(i32(4).expand(3, 4).contiguous(), i32(3))._c.table_stride == 4
+    assert ops.KVSeqs(i32(4)[None].expand(1, 4), i32(1))._c.table_stride == 0        # one row is one row
+    assert ops.KVSeqs(i32(3, 9)[:, :4], i32(3))._c.table_stride == 9
+    assert ops.KVSeqs(i32(3, 0), i32(3))._c.max_pages == 0
+    ctx = Ctx()
+    page = on_gpu(torch.zeros((1, 2, 16, 128), dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="k.contiguous"):
+        ops.KVCache(ctx, page.expand(5, -1, -1, -1), page.expand(5, -1, -1, -1))
+    assert ops.KVCache(ctx, page, page)._c.page_stride == 0
+    c, s = py_cache(on_gpu, ctx), ops.KVSeqs(i32(3, 4), i32(3))
+    q = on_gpu(torch.zeros((3, 1024)))
+    with pytest.raises(ValueError, match="out.contiguous"):
+        c.attend(s, q, out=on_gpu(torch.zeros(1024)).expand(3, 1024))
+    assert not ctx.calls
+    c.attend(s, q, out=on_gpu(torch.zeros((3, 2048)))[:, :1024])
+    assert ctx.calls[-1][1][-1] == 2048
+    # rows that are read may share memory: they are copied
+    c.attend(s, on_gpu(torch.zeros(1024)).expand(3, 1024), out=q)
+    assert ctx.calls[-1][1][5] == 1024 and ctx.calls[-1][1][4] % 16 == 0
+    c.append(s, on_gpu(torch.zeros(256)).expand(3, 256), on_gpu(torch.zeros((3, 256))))
+    assert ctx.calls[-1][1][5] == 256
+
+
 def test_the_64_bit_evaluation_against_differences():
     """The tests' own reference: rotation keeps lengths and composes, attention is the weighted mean of its definition."""
     import torch
