@@ -484,6 +484,12 @@ class Rope:
                                                  int(interleaved), C.byref(h)), "Rope")
         self._h = h
 
+    def handle(self) -> C.c_void_p:
+        """The C handle; NULL would mean "no rotation", so a closed one has none to give."""
+        if self._h is None:
+            raise ValueError("the rotation is closed")
+        return self._h
+
     def close(self) -> None:
         if getattr(self, "_h", None):
             self._lib.ferric_cuda_rope_free(self._h)
@@ -603,7 +609,7 @@ class KVCache:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {self.n_heads * self.head_dim}]")
         if seqs._dev != self._dev:
             raise ValueError(f"the sequences are on device {seqs._dev}, the context on device {self._dev}")
-        self._run(self._lib.ferric_cuda_kv_append, "kv_append", seqs._ref, rope._h if rope is not None else None, pk, ldk, pv, ldv, n)
+        self._run(self._lib.ferric_cuda_kv_append, "kv_append", seqs._ref, rope.handle() if rope is not None else None, pk, ldk, pv, ldv, n)
 
     def attend(self, seqs: KVSeqs, q: torch.Tensor, rope: Optional[Rope] = None, scale: Optional[float] = None, window: int = 0,
                out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -632,7 +638,7 @@ class KVCache:
         ty = GGML_F32 if out.dtype is torch.float32 else GGML_BF16
         if ty == GGML_BF16 and out.dtype is not torch.bfloat16:
             raise TypeError("the result is float32 or bfloat16")
-        self._run(self._lib.ferric_cuda_kv_attend, "kv_attend", seqs._ref, rope._h if rope is not None else None, pq, ldq, n,
+        self._run(self._lib.ferric_cuda_kv_attend, "kv_attend", seqs._ref, rope.handle() if rope is not None else None, pq, ldq, n,
                   cols // self.head_dim, scale, window, out.data_ptr(), ty, ldo)
         return out
 

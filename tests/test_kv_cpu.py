@@ -289,6 +289,31 @@ def test_expanded_tensors_are_refused(on_gpu):
     assert ctx.calls[-1][1][5] == 256
 
 
+def test_a_closed_rotation_is_refused(on_gpu):
+    """NULL means "as it is" in the C ABI: a closed rotation must not turn into none."""
+    import torch
+
+    from ferric_b200 import ops
+    ctx = Ctx()
+    c = py_cache(on_gpu, ctx)
+    s = ops.KVSeqs(on_gpu(torch.zeros((3, 4), dtype=torch.int32)), on_gpu(torch.zeros(3, dtype=torch.int32)))
+    q, k = on_gpu(torch.zeros((3, 1024))), on_gpu(torch.zeros((3, 256)))
+    rope = ops.Rope(ctx, 128)
+    rope._h = C.c_void_p(P)                                    # (the recording library made none)
+    c.append(s, k, k, rope=rope)
+    assert ctx.calls[-1][1][3].value == P
+    c.attend(s, q, out=q)
+    assert ctx.calls[-1][1][3] is None
+    rope.close()
+    rope.close()
+    n = len(ctx.calls)
+    with pytest.raises(ValueError, match="closed"):
+        c.append(s, k, k, rope=rope)
+    with pytest.raises(ValueError, match="closed"):
+        c.attend(s, q, rope=rope, out=q)
+    assert len(ctx.calls) == n
+
+
 def test_the_64_bit_evaluation_against_differences():
     """The tests' own reference: rotation keeps lengths and composes, attention is the weighted mean of its definition."""
     import torch
