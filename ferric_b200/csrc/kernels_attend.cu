@@ -342,11 +342,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 for (int e = t4; e < D; e += 4) mx = fmaxf(mx, fabsf(q[e]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                int e = 0;
-                if (mx > 0.0f && mx < INFINITY) frexpf(mx, &e);
-                e = min(max(e, -100), 100);
-                qscale = ldexpf(1.0f, 11 - e);
-                unscale = ldexpf(1.0f, e - 11);
+                f16_row_scale(mx, &qscale, &unscale);
             }
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {

@@ -14,8 +14,9 @@
 // -- only when the new one exceeds the old one by more than 2^kSlack; the division by the sum makes up for the rest.
 //
 // Rounding: the weights are rounded once to the cache's type (they multiply its values on the tensor cores; 2^-9 of a
-// weight in bf16, as much as the result's own rounding), summed in f32 before that.  q is rounded to f16 for an f16 cache; for
-// a bf16 cache it is split into two bf16 parts, since one alone would move every score by up to 2^-9 of its terms.
+// weight in bf16, as much as the result's own rounding), summed in f32 before that.  q is rounded to f16 for an f16 cache, each
+// row scaled by a power of two first (undone on its scores, in the subtraction of the maximum); for a bf16 cache it is split into
+// two bf16 parts, since one alone would move every score by up to 2^-9 of its terms.
 #include <string.h>
 
 #include <type_traits>
@@ -28,6 +29,12 @@ namespace ferric {
 int* gemm_status_word();   // device address of the status word shared with the tensor-core products (kernels_gemm.cu)
 int32_t encode_cache(CUtensorMap* map, const KvCacheView& c, void* base, const void* stand_in);   // kernels_attend.cu
 
+struct PromptBars {
+    uint64_t full[8], empty[8];
+    uint64_t s_full[2], p_full[2], pv_done[2], turn[2];
+    uint32_t tmem;
+    int tainted, last;
+};
 template <typename T, int D>
 struct PromptCfg {
     static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -46,23 +53,20 @@ struct PromptCfg {
     static constexpr int kThreads = kTrade ? 384 : 32 * (kSoftWarps + kMmaWarps + 1);
     static constexpr int kQBytes = kTilesQ * kParts * 128 * D * 2;
     static constexpr int kStageBytes = kKeys * D * 2;      // a tile of K or of V
-    static constexpr int kFixed = 1024 + 512 + kQBytes;
+    static constexpr int kBarBytes = 512;
+    static constexpr int kScaleBytes = kBf16 ? 0 : kRows * 4;   // f16: what undoes each row's scaling
+    static constexpr int kFixed = 1024 + kBarBytes + kScaleBytes + kQBytes;
     static constexpr int kStagesFit = (232448 - kFixed) / kStageBytes;
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static constexpr int kSmem = kFixed + kStages * kStageBytes;
     static constexpr int kOCol = 2 * kKeys;                // tensor memory: S0 | S1 | O (one per row tile)
     static constexpr int kPieceFloats = kRows * (D + 2);   // of a block whose keys several CTAs share: [D / 4][row][4], then m, l
+    static_assert(sizeof(PromptBars) <= kBarBytes, "barriers");
     static_assert(kStages >= 3 && kOCol + kTilesQ * D <= 512, "shared and tensor memory");
 };
 constexpr float kSlack = 6.0f;         // log2 units
 constexpr float kPromptShiftF16 = 8.0f;   // f16 weights are scaled by 2^8: at most 2^14 with the slack, normal down to 2^-22
 
-struct PromptBars {
-    uint64_t full[8], empty[8];
-    uint64_t s_full[2], p_full[2], pv_done[2], turn[2];
-    uint32_t tmem;
-    int tainted, last;
-};
 // Few blocks against many keys (a chunk of a prompt on a long cache) would leave most SMs idle: `splits` CTAs then share a
 // block's keys, each leaving a piece, and the last one joins them in order.
 struct PromptWork {
@@ -162,6 +166,12 @@ __device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi)
     return r;
 }
 __device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b)
 {
     uint64_t r;
@@ -193,6 +203,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     uint8_t* qs = smem;                              // [tile][part][D / 64][128 rows][128 bytes]
     uint8_t* ring = smem + C::kQBytes;               // [stage][D / 64][KT rows][128 bytes]
     PromptBars* bar = reinterpret_cast<PromptBars*>(ring + C::kStages * C::kStageBytes);
+    [[maybe_unused]] float* row_scale = reinterpret_cast<float*>(ring + C::kStages * C::kStageBytes + C::kBarBytes);   // f16: [row]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.heads / c.heads;
 
@@ -284,6 +295,18 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     uint8_t* base = qs + tile * (C::kParts * 128 * D * 2) + rr * 128;
 #pragma unroll
                     for (int e = 0; e < 16; e++) x[i][e] *= scale;
+                    if constexpr (!BF) {   // the row's largest magnitude: its units are in kUnits neighbouring lanes
+                        float mx = 0.0f, up, down;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) mx = fmaxf(mx, fabsf(x[i][e]));
+#pragma unroll
+                        for (int o = 1; o < kUnits; o <<= 1)
+                            mx = fmaxf(mx, __shfl_xor_sync(((1u << kUnits) - 1u) << (lane & ~(kUnits - 1)), mx, o));
+                        f16_row_scale(mx, &up, &down);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) x[i][e] *= up;
+                        if (u == 0) row_scale[row] = down;
+                    }
 #pragma unroll
                     for (int part = 0; part < C::kParts; part++) {
                         uint32_t w[8];
@@ -304,6 +327,9 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             }
         }
         // rows the block does not have
+        if constexpr (!BF) {
+            for (int i = b.rows + tid; i < C::kRows; i += 32 * C::kSoftWarps) row_scale[i] = 1.0f;
+        }
         for (int i = tid + b.rows * (D / 8); i < C::kRows * (D / 8); i += 32 * C::kSoftWarps) {
             const int row = i / (D / 8), ch = i % (D / 8);
 #pragma unroll
@@ -464,6 +490,8 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         const int lo_r = have ? kv_seen_lo(span.pos(j_tok), a.window) : 0, hi_r = have ? kv_seen_hi(c, s, span.pos(j_tok)) : 0;
         const int run = kv_min(KT == 128 ? 7 : 6, c.page_shift), pages = KT >> run;
         constexpr float kShift = BF ? 0.0f : kPromptShiftF16;
+        const float undo = BF ? 1.0f : row_scale[row];
+        const uint64_t undo2 = pack_f32x2(undo, undo);
         float m = -INFINITY, l = 0.0f;      // weights are 2^(s - m)
         for (int j = 0; j < tiles; j++) {
             const int u = j * NX + x, sb = u & 1, k0 = (t0 + j) * KT;
@@ -489,7 +517,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 #pragma unroll
             for (int i = 0; i < KT; i += 2)
                 asm("max.f32 %0, %0, %1, %2;" : "+f"(mq[(i >> 1) & 3]) : "f"(__uint_as_float(w[i])), "f"(__uint_as_float(w[i + 1])));
-            const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) - kShift;
+            const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * undo - kShift;
             // The products up to the unit before, complete.  A parity only tells neighbouring phases apart, so every phase is
             // waited for once, in order, and before this unit's weights are handed over: its own products cannot have
             // completed by then, and no later wait finds the barrier more than one phase away.
@@ -522,7 +550,8 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             uint64_t sum[2] = {0, 0};
 #pragma unroll
             for (int i = 0; i < KT / 2; i++) {
-                const uint64_t x = add_f32x2(pack_f32x2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])), minus);
+                const uint64_t s2 = pack_f32x2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+                const uint64_t x = BF ? add_f32x2(s2, minus) : fma_f32x2(s2, undo2, minus);
                 float p0, p1;
                 unpack_f32x2(x, p0, p1);
                 p0 = ex2_approx(p0);

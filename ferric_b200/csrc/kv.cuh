@@ -59,6 +59,17 @@ __device__ __forceinline__ void kv_from_float(float v, __nv_bfloat16* o) { *o = 
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The power of two that brings a row of q (in log2 units, largest magnitude `mx`) to f16's upper end, and its inverse: any finite
+// row fits f16 and keeps the type's 11 bits down to 2^-25 of its largest element, and undoing it on the scores is exact.
+__device__ __forceinline__ void f16_row_scale(float mx, float* up, float* down)
+{
+    int e = 0;
+    if (mx > 0.0f && mx < INFINITY) frexpf(mx, &e);
+    e = max(e, -100);
+    *up = ldexpf(1.0f, 11 - e);
+    *down = ldexpf(1.0f, e - 11);
+}
+
 // One query row against keys [lo, hi) of one sequence and head, by one warp, in f32: the definition, key by key.  `q` is
 // the rotated row times scale * log2(e), in shared memory.  Lane = key for the scores, lane = dimension for the sums, so a
 // masked or absent key is never multiplied by anything.  Leaves the running maximum (log2 units), the sum and the

@@ -288,6 +288,18 @@ def test_prompt_scales(F, ctx, dtype, scale):
     Batch(F, ctx, lens=[700], new=[140], heads=2, kv_heads=1, page=64, dtype=dtype).check_attend(out_dtype=BF, scale=scale)
 
 
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q,k,scale", [(2.0 ** 20, 2.0 ** -20, None), (1.0, 2.0 ** 12, 2.0 ** -16), (2.0 ** -30, 2.0 ** 12, 2.0 ** 14), (2.0 ** 100, 0.0, None)])
+def test_prompt_of_any_finite_size(F, ctx, out_dtype, dtype, dim, q, k, scale):
+    """scale * q far outside f16's range on either side, against keys that bring the scores back to ordinary ones (or are 0)."""
+    b = Batch(F, ctx, lens=[300, 90], new=[140, 90], heads=5, kv_heads=1, dim=dim, page=64, dtype=dtype)
+    b.q.mul_(q)
+    b.cache.k.mul_(k)
+    b.check_attend(out_dtype=out_dtype, scale=scale)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("lens,new", [([900], [900]), ([1500, 333], [130, 70])])
