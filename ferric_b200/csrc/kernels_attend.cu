@@ -504,6 +504,9 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         // the row's halves and the quad's sums together
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
+        // An infinite key: the score of q in parts is inf - inf or 0 inf where that of q itself may be -inf, a weight of 0.  The sum of
+        // the weights shows it, and such a block is done again too.
+        if (l != l && my_r < b.rows) bar->tainted = 1;
         float2 oo[NT];
 #pragma unroll
         for (int i = 0; i < NT; i++) oo[i] = make_float2(o[i][0] + o[i][2], o[i][1] + o[i][3]);
@@ -550,8 +553,8 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 
         // now the kn == 0 warps hold their tile's rows: lane (g, t) elements 8 i + 2 t + {0, 1} of row g
         if (tainted) {
-            // A value that some rows of the block see and others do not is not finite: weight 0 does not hide it in a matrix
-            // product.  The rows again, one by one and key by key, over this CTA's tiles of the block.
+            // A value that some rows of the block see and others do not is not finite -- weight 0 does not hide it in a matrix
+            // product -- or a row's weights are NaN.  The rows again, one by one and key by key, over this CTA's tiles of the block.
             named_bar_sync(1, kCons);
             for (int r = warp; r < b.rows; r += C::kWarps) {
                 float* q = buf + r * C::kPitch;   // the row's q, then its results

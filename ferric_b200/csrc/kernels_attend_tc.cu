@@ -573,6 +573,8 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
         wait(&bar->pv_done[x], (tiles - 1) & 1, 57);
         tc_fence_after();
+        // an infinite key: q's parts (or an element rounded to 0) make inf - inf or 0 inf of what may be a score of -inf
+        if (have && l != l) bar->tainted = 1;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         // The result goes through the tile's place of Q, done with since its last S: written row by row as tensor memory
         // holds it (16-byte chunks, permuted so that eight rows do not meet in a bank), stored row-contiguously.

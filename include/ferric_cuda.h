@@ -376,7 +376,8 @@ int32_t ferric_cuda_kv_append(ferric_cuda_ctx *ctx, const ferric_kv_cache *cache
  * out is FERRIC_GGML_F32 (the decode products' activation type: the whole product is then kept to f32 accuracy) or
  * FERRIC_GGML_BF16 (the prefill products'), 16-byte aligned with row stride ldo (0 = dense; a multiple of 16 bytes), and
  * must not overlap q (refused).  A token that sees no key gets zeros; output rows outside every sequence are left as they were.  The
- * new tokens' own keys must have been appended.  A key or value element that is not finite reaches only the tokens that see it.
+ * new tokens' own keys must have been appended.  A key or value element that is not finite reaches only the tokens that see it;
+ * a key with a score of -inf weighs nothing (such infinities come of an append to f16 of numbers above 65504).
  * Calls on one context share a workspace (ferric_cuda_attend_reserve, allocated by the first call otherwise, which must then
  * not be under capture): graphs captured on one context must not be replayed at the same time -- give each stream of
  * replays a context of its own.  Waits inside the kernels are bounded; ferric_cuda_gemm_status reports one that ran out. */

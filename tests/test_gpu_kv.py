@@ -357,6 +357,29 @@ def test_what_is_not_finite_reaches_only_the_tokens_that_see_it(F, ctx, out_dtyp
         assert fine[sees][:, 2:][..., keep].all()
 
 
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens,new", [([200, 70, 9], None), ([200, 300], [5, 3]), ([300, 150], [140, 150]), ([2600], [57])])
+def test_an_infinite_key_with_a_score_of_minus_infinity_weighs_nothing(F, ctx, out_dtype, dtype, dim, lens, new):
+    """Every query has a negative element where 16 keys hold an infinity: their scores are -inf, as if the keys were not there."""
+    b = Batch(F, ctx, lens=lens, new=new, heads=5, kv_heads=1, dim=dim, page=16, dtype=dtype, rotary=0)
+    b.q[:, 5::dim] = -b.q[:, 5::dim].abs() - 0.1
+    b.q[:, 6::dim] = 1.0                                       # exact in one part: the others are 0
+    there = b.table.clone()
+    for i in range(len(lens)):
+        c = min(2, (lens[i] - 1) // 16)
+        pg = int(there[i, c])
+        b.cache.k[pg, 0, :, 5] = float("inf")
+        b.cache.k[pg, 0, :, 6] = float("-inf")
+        b.table[i, c] = -1                                     # for the reference: not there
+    y = b.cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=out_dtype).double().cpu()
+    want, bound, mine = R.attend(b.cache.k, b.cache.v, b.table, b.lens, b.starts, b.q, b.heads, b.rope_ref, out_dtype=out_dtype)
+    assert torch.isfinite(y).all()
+    assert ((y - want).abs() <= bound).all()
+    b.check_rows(y, want, mine, out_dtype)
+
+
 def test_value_outside_the_window_does_not_leak(F, ctx):
     b = Batch(F, ctx, lens=[200, 200], new=[1, 40], heads=4, kv_heads=1, page=16)
     for i in range(2):
