@@ -372,12 +372,40 @@ int32_t ferric_cuda_ctx_create(int device, ferric_cuda_ctx** out)
     return kOk;
 }
 
+// Order `to` behind the attention still running on the context's stream.  Work under capture does not run, and a capture must
+// not wait for work outside it: such a stream is passed over, and the one set after it waits.
+static int32_t follow_attention(ferric_cuda_ctx* ctx, cudaStream_t to)
+{
+    if (!ctx->attend_event || to == ctx->stream) return kOk;
+    auto capturing = [](cudaStream_t s) {
+        cudaStreamCaptureStatus c = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(s, &c) == cudaSuccess) return c != cudaStreamCaptureStatusNone;
+        cudaGetLastError();   // (the legacy stream, while a capture forbids its use)
+        return true;
+    };
+    DeviceGuard guard(ctx->device);
+    if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
+    if (ctx->attend_used && !capturing(ctx->stream)) {
+        if (ctx->attend_pending) FERRIC_CUDA_TRY(cudaStreamWaitEvent(ctx->stream, ctx->attend_event, 0));
+        FERRIC_CUDA_TRY(cudaEventRecord(ctx->attend_event, ctx->stream));
+        ctx->attend_pending = true;
+    }
+    ctx->attend_used = false;
+    if (ctx->attend_pending && !capturing(to)) {
+        FERRIC_CUDA_TRY(cudaStreamWaitEvent(to, ctx->attend_event, 0));
+        ctx->attend_pending = false;
+    }
+    return kOk;
+}
+
 int32_t ferric_cuda_ctx_set_stream(ferric_cuda_ctx* ctx, void* cuda_stream)
 {
     if (!ctx) {
         set_last_error("NULL context");
         return kErrInvalidArg;
     }
+    const int32_t rc = follow_attention(ctx, reinterpret_cast<cudaStream_t>(cuda_stream));
+    if (rc != kOk) return rc;
     if (ctx->owns_stream) {
         DeviceGuard guard(ctx->device);
         cudaStreamSynchronize(ctx->stream);
@@ -409,6 +437,7 @@ void ferric_cuda_ctx_free(ferric_cuda_ctx* ctx)
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->tune.split_ws.partial) cudaFree(ctx->tune.split_ws.partial);
     if (ctx->attend_ws) cudaFree(ctx->attend_ws);
+    if (ctx->attend_event) cudaEventDestroy(ctx->attend_event);
     if (ctx->owns_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
 }

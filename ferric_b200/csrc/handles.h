@@ -29,6 +29,10 @@ struct ferric_cuda_ctx {
     unsigned* chain_tickets = nullptr;
     unsigned* chain_done = nullptr;
     void* attend_ws = nullptr;   // pieces of rows that several CTAs attend to, and their tickets (ferric_cuda_attend_reserve)
+    // The workspace is the context's, whatever stream its calls go to; another stream is ordered behind its last use.
+    cudaEvent_t attend_event = nullptr;
+    bool attend_used = false;      // on `stream`, since that was set
+    bool attend_pending = false;   // the event is recorded and `stream`, under capture when it was set, could not wait for it
 };
 
 struct ferric_qmatrix {

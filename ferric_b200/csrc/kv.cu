@@ -252,6 +252,7 @@ int32_t ferric_cuda_attend_reserve(ferric_cuda_ctx* ctx)
         set_last_error("the attention's workspace is not allocated yet: call ferric_cuda_attend_reserve (or attend once) before capturing");
         return kErrInvalidArg;
     }
+    if (!ctx->attend_event) FERRIC_CUDA_TRY(cudaEventCreateWithFlags(&ctx->attend_event, cudaEventDisableTiming));
     void* ws = nullptr;
     FERRIC_CUDA_TRY(cudaMalloc(&ws, attend_ws_bytes(ctx->tune.sm_count)));
     cudaError_t e = cudaMemsetAsync(ws, 0, attend_ticket_bytes(), ctx->stream);
@@ -321,7 +322,10 @@ int32_t ferric_cuda_kv_attend(ferric_cuda_ctx* ctx, const ferric_kv_cache* cache
     if ((rc = ferric_cuda_attend_reserve(ctx)) != kOk) return rc;
     int launched = 0;
     rc = launch_attend(ctx->stream, c, s, r, a, ctx->attend_ws, ctx->tune, &launched);
-    if (rc == kOk) ctx->launches += launched;
+    if (rc == kOk) {
+        ctx->launches += launched;
+        ctx->attend_used = true;
+    }
     return rc;
 }
 

@@ -72,7 +72,9 @@ int32_t ferric_cuda_ctx_create(int device, ferric_cuda_ctx **out);
 /* Same, but launches go to a caller-owned stream (cudaStream_t passed as void*; NULL = the
  * legacy default stream), e.g. the stream of the framework hosting the activations. */
 int32_t ferric_cuda_ctx_create_on_stream(int device, void *cuda_stream, ferric_cuda_ctx **out);
-/* Redirect later launches to another stream of the same device. */
+/* Redirect later launches to another stream of the same device.  The caller orders the new stream behind the old one where work
+ * is still running there (the activation scratch is the context's); once the context has attended (ferric_cuda_kv_attend) this
+ * call does so itself, and the old stream must still exist. */
 int32_t ferric_cuda_ctx_set_stream(ferric_cuda_ctx *ctx, void *cuda_stream);
 void *ferric_cuda_ctx_stream(const ferric_cuda_ctx *ctx);
 /* Block until everything queued on the context's stream is done (the reference's
@@ -379,8 +381,8 @@ int32_t ferric_cuda_kv_append(ferric_cuda_ctx *ctx, const ferric_kv_cache *cache
  * new tokens' own keys must have been appended.  A key or value element that is not finite reaches only the tokens that see it;
  * a key with a score of -inf weighs nothing (such infinities come of an append to f16 of numbers above 65504).
  * Calls on one context share a workspace (ferric_cuda_attend_reserve, allocated by the first call otherwise, which must then
- * not be under capture): graphs captured on one context must not be replayed at the same time -- give each stream of
- * replays a context of its own.  Waits inside the kernels are bounded; ferric_cuda_gemm_status reports one that ran out. */
+ * not be under capture): graphs captured on one context must not be replayed at the same time, nor beside its other calls
+ * -- give each stream of replays a context of its own.  Waits inside the kernels are bounded; ferric_cuda_gemm_status reports one that ran out. */
 int32_t ferric_cuda_kv_attend(ferric_cuda_ctx *ctx, const ferric_kv_cache *cache, const ferric_kv_seqs *seqs, const ferric_rope *rope,
                               const float *q_dev, size_t ldq, size_t n_tokens, size_t n_q_heads, float scale, size_t window,
                               void *out_dev, uint32_t out_type, size_t ldo);

@@ -546,6 +546,42 @@ def test_two_contexts_on_two_streams(F):
         r[1].close()
 
 
+def test_a_context_that_changes_streams(F, ctx):
+    """Calls on one stream still running when the context is given another: they share the workspace, so the second waits."""
+    many = [Batch(F, ctx, lens=[20000, 9000 + 1000 * i], heads=8, kv_heads=1, page=64, seed=i) for i in range(3)]
+    prompt = Batch(F, ctx, lens=[2600], new=[57], heads=5, kv_heads=1, page=32, seed=5)
+    want = [b.cache.attend(b.seqs, b.q, rope=b.rope).clone() for b in many]
+    want_p = prompt.cache.attend(prompt.seqs, prompt.q, rope=prompt.rope, out_dtype=BF).clone()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    a = torch.randn((4096, 4096), device="cuda")
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(9):
+        with torch.cuda.stream(streams[turn % 3]):
+            ctx.use_torch_stream()
+            if turn == 0:
+                for _ in range(20):                            # the first stream is late
+                    a = a @ a * 1e-3
+            for i, b in enumerate(many):
+                got.append((want[i], b.cache.attend(b.seqs, b.q, rope=b.rope)))
+            got.append((want_p, prompt.cache.attend(prompt.seqs, prompt.q, rope=prompt.rope, out_dtype=BF)))
+    # a capture in between neither waits nor is waited for; what comes after it waits for what ran before it
+    g = torch.cuda.CUDAGraph()
+    out = torch.empty_like(want[0])
+    with torch.cuda.graph(g, stream=streams[1]):
+        ctx.use_torch_stream()
+        many[0].cache.attend(many[0].seqs, many[0].q, rope=many[0].rope, out=out)
+    with torch.cuda.stream(streams[0]):
+        ctx.use_torch_stream()
+        got.append((want[1], many[1].cache.attend(many[1].seqs, many[1].q, rope=many[1].rope)))
+        g.replay()
+    torch.cuda.synchronize()
+    got.append((want[0], out))
+    ctx.use_torch_stream()
+    for w, y in got:
+        assert torch.equal(w, y)
+
+
 def test_context_with_a_stream_of_its_own(F):
     c = F.Context(0, stream=None)
     b = Batch(F, c, lens=[100, 9], new=[4, 9], fill=False)
