@@ -194,13 +194,22 @@ int32_t ferric_cuda_rope_create(ferric_cuda_ctx* ctx, size_t rotary, double base
     }
     DeviceGuard guard(ctx->device);
     if (!guard.ok) return cuda_fail(cudaGetLastError(), "cudaSetDevice");
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    FERRIC_CUDA_TRY(cudaStreamIsCapturing(ctx->stream, &cap));
+    if (cap != cudaStreamCaptureStatusNone) {
+        set_last_error("a rotation allocates and synchronises: create it before capturing");
+        return kErrInvalidArg;
+    }
     ferric_rope* r = new (std::nothrow) ferric_rope;
     if (!r) return kErrOom;
     r->device = ctx->device;
     r->rotary = (int)rotary;
     r->interleaved = interleaved != 0;
     cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&r->turns), sizeof(double) * (rotary / 2));
-    if (e == cudaSuccess) e = cudaMemcpy(r->turns, turns, sizeof(double) * (rotary / 2), cudaMemcpyHostToDevice);
+    // The copy is waited for on its stream: cudaMemcpy from pageable memory may return with the transfer to the device still
+    // to come, and the streams that use the rotation are not ordered behind it.
+    if (e == cudaSuccess) e = cudaMemcpyAsync(r->turns, turns, sizeof(double) * (rotary / 2), cudaMemcpyHostToDevice, ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     if (e != cudaSuccess) {
         if (r->turns) cudaFree(r->turns);
         delete r;

@@ -150,6 +150,31 @@ def test_append_takes_given_frequencies(F, ctx):
     check_append(b)
 
 
+def test_a_rotation_is_there_when_it_has_been_made(F):
+    """Made and used at once, on streams that nothing orders; refused under capture, which stays usable."""
+    c = F.Context(0, stream=None)
+    b = Batch(F, c, lens=[70, 9], new=[30, 9], fill=False)
+    torch.cuda.synchronize()
+    for i in range(30):
+        b.rope_ref = dict(rotary=128, base=1000.0 + i)
+        b.rope = F.Rope(c, 128, base=1000.0 + i)
+        check_append(b)
+    out = torch.zeros(4, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    c.set_stream(side.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        out.add_(1.0)
+        with pytest.raises(F.FerricError, match="before capturing"):
+            F.Rope(c, 128)
+        out.add_(1.0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert (out == 2.0).all()
+    c.close()
+
+
 # ---- attend: one new token per sequence ----------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("dim", [64, 128, 256])
