@@ -575,26 +575,47 @@ class KVCache:
         if x.dim() == 3:
             if x.shape[2] != self.head_dim:
                 raise ValueError(f"{name} has heads of {x.shape[2]}, the cache of {self.head_dim}")
-            x = x.flatten(1) if x.stride(2) == 1 and (x.shape[1] <= 1 or x.stride(1) == self.head_dim) else x.contiguous().flatten(1)
+            x = x.flatten(1) if x.stride(2) == 1 and (x.shape[1] <= 1 or x.stride(1) == self.head_dim) else self._dense(x).flatten(1)
         elif x.dim() != 2:
             raise TypeError(f"{name} must have two or three dimensions, not {x.dim()}")
         n, cols = x.shape
         ld, step = x.stride()
         p = x.data_ptr()
         if (step != 1 and cols > 1) or (n > 1 and (ld < cols or ld % 4)) or p % 16:
-            x = x.contiguous()
+            x = self._dense(x)
             ld, p = cols, x.data_ptr()
         return x, n, cols, p, ld if n > 1 else 0
+
+    def _streams(self):
+        """(torch's current stream, the context's), or None where they are one."""
+        st = self.ctx._stream
+        if st == torch._C._cuda_getCurrentRawStream(self._dev):
+            return None
+        own = torch.cuda.ExternalStream(st, device=self._dev) if st else torch.cuda.default_stream(self._dev)
+        return torch.cuda.current_stream(self._dev), own
+
+    def _dense(self, x: torch.Tensor) -> torch.Tensor:
+        """A dense copy, made on torch's stream: behind what the context's may still have to write into `x` (a product's result).
+        A capture that the context's stream is not part of has nothing there to wait for, and must not wait for what is."""
+        two = self._streams()
+        if two is not None:
+            cur, own = two
+            with torch.cuda.stream(cur):
+                capture = torch.cuda.is_current_stream_capturing()
+            with torch.cuda.stream(own):
+                capture = capture and not torch.cuda.is_current_stream_capturing()
+            if not capture:
+                cur.wait_stream(own)
+        return x.contiguous()
 
     def _run(self, fn, where: str, *args) -> None:
         """The call on the context's stream.  Where that is not torch's current one, it waits for what torch has queued there and
         what torch queues next waits for it, so operands and results may be made and dropped as if it ran on that stream."""
-        st = self.ctx._stream
-        if st == torch._C._cuda_getCurrentRawStream(self._dev):
+        two = self._streams()
+        if two is None:
             _check(fn(self.ctx._h, self._ref, *args), where)
             return
-        cur = torch.cuda.current_stream(self._dev)
-        own = torch.cuda.ExternalStream(st, device=self._dev) if st else torch.cuda.default_stream(self._dev)
+        cur, own = two
         own.wait_stream(cur)
         try:
             _check(fn(self.ctx._h, self._ref, *args), where)

@@ -620,6 +620,41 @@ def test_context_with_a_stream_of_its_own(F):
     c.close()
 
 
+def test_copied_operands_wait_for_the_contexts_stream(F):
+    """An operand that has to be copied, still being written on the context's own stream when the call is made."""
+    c = F.Context(0, stream=None)
+    b = Batch(F, c, lens=[50, 60, 70], page=32, fill=False)
+    b.cache.k.zero_(), b.cache.v.zero_()
+    own = torch.cuda.ExternalStream(c._lib.ferric_cuda_ctx_stream(c._h))
+    wide = torch.zeros((3, b.qkv.shape[1] + 7), device="cuda")
+    odd = wide[:, 5:5 + b.qkv.shape[1]]                         # neither aligned nor a stride of four
+    q, k, v = odd[:, :1024], odd[:, 1024:1280], odd[:, 1280:]
+    apart = torch.zeros((3, 8, 2, 128), device="cuda")
+    a = torch.randn((4096, 4096), device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(own):
+        for _ in range(20):
+            a = a @ a * 1e-3
+        odd.copy_(b.qkv)
+        apart[:, :, 0] = b.q.reshape(3, 8, 128)
+    b.cache.append(b.seqs, k, v, rope=b.rope)
+    y = [b.cache.attend(b.seqs, x, rope=b.rope) for x in (q, apart[:, :, 0])]
+    # under capture: the copy is captured, and nothing waits for what is outside
+    side, out = torch.cuda.Stream(), torch.empty_like(y[0])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        b.cache.attend(b.seqs, q, rope=b.rope, out=out)
+        b.cache.attend(b.seqs, q, rope=b.rope, out=out)
+    g.replay()
+    torch.cuda.synchronize()
+    want, bound, _ = R.attend(b.cache.k, b.cache.v, b.table, b.lens, None, b.q, 8, b.rope_ref)
+    for x in (*y, out):
+        assert ((x.double().cpu() - want).abs() <= bound).all()
+    assert b.cache.k.count_nonzero() > 3 * 2 * 100
+    c.close()
+
+
 def test_operands_that_are_not_dense(F, ctx):
     """3-D views, odd strides and offsets: taken in place or copied, never misread."""
     b = Batch(F, ctx, lens=[50, 60, 70], page=32)

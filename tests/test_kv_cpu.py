@@ -247,6 +247,7 @@ def on_gpu(monkeypatch):
         ops._check(fn(self.ctx._h, self._ref, *args), where)
 
     monkeypatch.setattr(ops.KVCache, "_run", run)
+    monkeypatch.setattr(ops.KVCache, "_streams", lambda self: None, raising=False)
     return lambda t: t.as_subclass(OnGpu)
 
 
