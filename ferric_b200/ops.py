@@ -645,8 +645,8 @@ class KVCache:
             raise ValueError("window must not be negative")
         if scale is None:
             scale = 0.0
-        elif scale == 0.0:
-            raise ValueError("scale must not be 0 (None = 1 / sqrt(head_dim))")
+        elif C.c_float(scale).value == 0.0:          # as the C ABI gets it, where 0 means the default
+            raise ValueError("scale must not be 0 in 32 bits (None = 1 / sqrt(head_dim))")
         if seqs._dev != self._dev:
             raise ValueError(f"the sequences are on device {seqs._dev}, the context on device {self._dev}")
         if out is None:

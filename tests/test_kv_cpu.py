@@ -315,6 +315,24 @@ def test_a_closed_rotation_is_refused(on_gpu):
     assert len(ctx.calls) == n
 
 
+def test_a_scale_that_is_0_in_32_bits_is_refused(on_gpu):
+    """0 means 1 / sqrt(head_dim) in the C ABI: a scale that rounds to it must not become that."""
+    import torch
+
+    from ferric_b200 import ops
+    ctx = Ctx()
+    c = py_cache(on_gpu, ctx)
+    s = ops.KVSeqs(on_gpu(torch.zeros((3, 4), dtype=torch.int32)), on_gpu(torch.zeros(3, dtype=torch.int32)))
+    q = on_gpu(torch.zeros((3, 1024)))
+    for scale in (0.0, -0.0, 1e-46, -1e-60):
+        with pytest.raises(ValueError, match="scale"):
+            c.attend(s, q, scale=scale, out=q)
+    assert not ctx.calls
+    c.attend(s, q, scale=1e-44, out=q)
+    c.attend(s, q, out=q)
+    assert ctx.calls[0][1][8] == 1e-44 and ctx.calls[1][1][8] == 0.0
+
+
 def test_the_64_bit_evaluation_against_differences():
     """The tests' own reference: rotation keeps lengths and composes, attention is the weighted mean of its definition."""
     import torch
