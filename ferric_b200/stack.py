@@ -158,6 +158,7 @@ class DecodeStack:
         self.rope = Rope(self.ctx, rotary, a.rope_base, a.interleaved) if rotary else None
         self.caches = [KVCache.empty(self.ctx, B * pages, a.page_size, p.kv_rows // d, d, a.dtype) for _ in range(self.n_layers)]
         self.att = torch.empty((B, p.q_rows), dtype=torch.float32, device=dev)
+        self.ctx.attend_reserve()       # now, so that a first step may be a captured one
         self.longest = 0        # tokens in the longest sequence, kept on the host beside the device's lengths
 
     def set_lengths(self, lens) -> None:
@@ -336,23 +337,31 @@ class DecodeStack:
             lens, longest = self.seqs.lens.clone(), self.longest
             self.longest = -warmup - 1
             self.seqs.lens.fill_(self.longest)
+        try:
+            self.graph = self._record(warmup)
+        finally:                # the lengths come back whatever became of it
+            if self.attention is not None:
+                self.seqs.lens.copy_(lens)
+                self.longest = longest
+
+    def _record(self, warmup: int) -> torch.cuda.CUDAGraph:
         side = torch.cuda.Stream(device=self.ctx.device)
         side.wait_stream(torch.cuda.current_stream(self.ctx.device))
-        with torch.cuda.stream(side):
-            self.ctx.use_torch_stream()
-            for _ in range(warmup):
+        try:
+            with torch.cuda.stream(side):
+                self.ctx.use_torch_stream()
+                for _ in range(warmup):
+                    self.step()
+            torch.cuda.current_stream(self.ctx.device).wait_stream(side)
+            torch.cuda.synchronize(self.ctx.device)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                self.ctx.use_torch_stream()
                 self.step()
-        torch.cuda.current_stream(self.ctx.device).wait_stream(side)
-        torch.cuda.synchronize(self.ctx.device)
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        finally:
+            torch.cuda.current_stream(self.ctx.device).wait_stream(side)
             self.ctx.use_torch_stream()
-            self.step()
-        self.ctx.use_torch_stream()
-        if self.attention is not None:
-            self.seqs.lens.copy_(lens)
-            self.longest = longest
-        self.graph = g
+        return g
 
     def run(self) -> torch.Tensor:
         if self.graph is not None:

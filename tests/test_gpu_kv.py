@@ -802,6 +802,37 @@ def test_stack_with_attention(F, ctx, batch):
     st.close()
 
 
+def test_stack_captured_before_anything_has_run(F):
+    """capture(warmup=0) as the context's first attention, and a capture that fails: the lengths are what they were."""
+    c = F.Context(0)
+    st = stack_of(F, c, 2)
+    st.set_lengths([5, 0])
+    st.capture(warmup=0)
+    assert st.seqs.lens.tolist() == [5, 0] and st.longest == 5
+    st.h.normal_()
+    st.run()
+    assert st.seqs.lens.tolist() == [6, 1]
+    c2 = F.Context(0)
+    broken = stack_of(F, c2, 2)
+    broken.set_lengths([7, 3])
+    stream, mix = c2._stream, broken._mix
+
+    def fails(i):
+        raise RuntimeError("stopped")
+    broken._mix = fails
+    with pytest.raises(RuntimeError, match="stopped"):
+        broken.capture()
+    assert broken.seqs.lens.tolist() == [7, 3] and broken.longest == 7 and broken.graph is None and c2._stream == stream
+    broken._mix = mix
+    broken.h.normal_()
+    broken.capture()
+    broken.run()
+    assert broken.seqs.lens.tolist() == [8, 4]
+    torch.cuda.synchronize()
+    for x in (st, broken, c, c2):
+        x.close()
+
+
 def test_stack_refuses_what_it_cannot_hold(F, ctx):
     from ferric_b200.stack import Attention, DecodeStack, TPPlan
     st = stack_of(F, ctx, 2)
