@@ -74,6 +74,7 @@ struct SplitBars {
     long long warp_sum[16];
     long long item_start;
     int seq, tainted, last;
+    volatile int abort;          // a wait ran out
 };
 
 __device__ __forceinline__ float ex2f(float x)
@@ -156,7 +157,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         }
         mbar_init(&bar->q_full, 1);
         mbar_init(&bar->q_empty, C::kWarps);
-        bar->tainted = 0;
+        bar->tainted = bar->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_launch_dependents();
@@ -258,7 +259,12 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     auto wait = [&](uint64_t* which, uint32_t parity, int code) {
         if (dead || mbar_wait(which, parity)) return;
         dead = true;
+        bar->abort = code;
         if (wk.status) atomicExch(wk.status, code);
+    };
+    auto let_copies_land = [&] {              // .. before the CTA's memory goes away
+        if (!bar->abort) return;
+        for (int i = 0; i < 200; i++) __nanosleep(1000);
     };
 
     if (warp == C::kWarps) {
@@ -271,6 +277,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             const int ta = item < x0 ? (int)(x0 - item) : 0, tb = item + b.tiles > x1 ? (int)(x1 - item) : b.tiles;
             // the block's q rows come before its tiles, so that they are not queued behind a ring full of them
             if (nq > 0) wait(&bar->q_empty, (nq - 1) & 1, 42);
+            if (__any_sync(0xffffffffu, dead)) break;   // its place may still be in use
             nq++;
             if (lane == 0) mbar_expect_tx(&bar->q_full, (uint32_t)b.rows * D * 4);
             __syncwarp();
@@ -284,6 +291,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 const int page = kv_page(c, s, seq, pos >> c.page_shift);
                 const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
                 if (n >= C::kStages) wait(&bar->empty[st], ((n / C::kStages) & 1) ^ 1, 40);
+                if (__any_sync(0xffffffffu, dead)) break;
                 if (lane == 0) {
                     bar->valid[st] = have & ((1u << pp) - 1u);
                     mbar_expect_tx(&bar->full[st], C::kStageBytes);
@@ -297,6 +305,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 }
             }
         }
+        let_copies_land();
         return;
     }
 
@@ -693,6 +702,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
         }
     }
+    let_copies_land();
 }
 
 // ---------------------------------------------------------------------------------------------------------------------

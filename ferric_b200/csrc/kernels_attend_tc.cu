@@ -34,6 +34,7 @@ struct PromptBars {
     uint64_t s_full[2], p_full[2], pv_done[2], turn[2];
     uint32_t tmem;
     int tainted, last;
+    volatile int abort;   // a wait ran out
 };
 template <typename T, int D>
 struct PromptCfg {
@@ -255,7 +256,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             mbar_init(&bar->pv_done[i], 1);
             mbar_init(&bar->turn[i], 1);
         }
-        bar->tainted = 0;
+        bar->tainted = bar->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // Q: rotated, scaled to log2 units, in 16-bit parts, K-major with a 128-byte swizzle.  A thread takes one token's 16
@@ -346,6 +347,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     auto wait = [&](uint64_t* which, uint32_t parity, int code) {
         if (dead || mbar_wait(which, parity)) return;
         dead = true;
+        bar->abort = code;
         if (wk.status) atomicExch(wk.status, code);
     };
     // keys every row of the block sees: tiles inside need no mask
@@ -362,12 +364,13 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             const int st = n % C::kStages, pos = (t0 + j) * KT + piece * box;
             const int page = kv_page(c, s, seq, pos >> c.page_shift);
             if (n >= C::kStages) wait(&bar->empty[st], ((n / C::kStages) & 1) ^ 1, 50);
+            n++;
+            if (__any_sync(0xffffffffu, dead)) return;   // its place may still be in use
             if (lane == 0) mbar_expect_tx(&bar->full[st], C::kStageBytes);
             __syncwarp();
             if (lane < copies)
                 tma_load_4d(ring + st * C::kStageBytes + half * (KT * 128) + piece * box * 128, map, half * 64, pos & ((1 << c.page_shift) - 1), head,
                             page >= 0 ? page : max(1, c.n_pages), &bar->full[st]);
-            n++;
         };
         for (int j = 0; j < kv_min(PRE, tiles); j++) load(&kmap, j);
         for (int j = 0; j < tiles; j++) {
@@ -622,6 +625,10 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
     }
     __syncthreads();
+    if (bar->abort) {
+        for (int i = 0; i < 200; i++) __nanosleep(1000);   // let copies and products still in flight finish
+        __syncthreads();
+    }
     if (warp == C::kSoftWarps)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     if (bar->tainted) {
