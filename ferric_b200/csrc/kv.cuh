@@ -63,11 +63,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // row fits f16 and keeps the type's 11 bits down to 2^-25 of its largest element, and undoing it on the scores is exact.
 __device__ __forceinline__ void f16_row_scale(float mx, float* up, float* down)
 {
-    int e = 0;
-    if (mx > 0.0f && mx < INFINITY) frexpf(mx, &e);
-    e = max(e, -100);
-    *up = ldexpf(1.0f, 11 - e);
-    *down = ldexpf(1.0f, e - 11);
+    // mx < 2^e, from its exponent bits; rows of less than 2^-100 keep that scaling, and one with an infinity stays infinite
+    const int e = max((int)(__float_as_uint(mx) >> 23) - 126, -100);
+    *up = __uint_as_float((unsigned)(127 + 11 - e) << 23);
+    *down = __uint_as_float((unsigned)(127 - 11 + e) << 23);
 }
 
 // One query row against keys [lo, hi) of one sequence and head, by one warp, in f32: the definition, key by key.  `q` is
