@@ -472,7 +472,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     umma_commit(&bar->s_full[buffer(j + PRE)]);
                     umma_commit(&bar->empty[sk]);
                 }
-                umma_commit(&bar->pv_done[x]);
+                if (PRE == 2 || !more) umma_commit(&bar->pv_done[x]);
             }
             __syncwarp();
         }
@@ -521,10 +521,11 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             for (int i = 0; i < KT; i += 2)
                 asm("max.f32 %0, %0, %1, %2;" : "+f"(mq[(i >> 1) & 3]) : "f"(__uint_as_float(w[i])), "f"(__uint_as_float(w[i + 1])));
             const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * undo - kShift;
-            // The products up to the unit before, complete.  A parity only tells neighbouring phases apart, so every phase is
-            // waited for once, in order, and before this unit's weights are handed over: its own products cannot have
-            // completed by then, and no later wait finds the barrier more than one phase away.
-            bool summed = j == 0;
+            // O may be touched once the unit before has been added.  Where S runs one unit ahead, S itself says so: its commit
+            // covers what the thread issued before.  Where it runs two ahead, pv_done does.  A parity only tells neighbouring
+            // phases apart, so every phase of that is waited for once, in order, and before this unit's weights are handed
+            // over: its own products cannot have completed by then, and no wait finds the barrier more than one phase away.
+            bool summed = PRE == 1 || j == 0;
             auto wait_summed = [&] {
                 if (!summed) wait(&bar->pv_done[x], (j - 1) & 1, 56);
                 summed = true;
@@ -574,7 +575,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->p_full[sb]);
         }
-        wait(&bar->pv_done[x], (tiles - 1) & 1, 57);
+        wait(&bar->pv_done[x], PRE == 2 ? (tiles - 1) & 1 : 0, 57);
         tc_fence_after();
         // an infinite key: q's parts (or an element rounded to 0) make inf - inf or 0 inf of what may be a score of -inf
         if (have && l != l) bar->tainted = 1;
