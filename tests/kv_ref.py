@@ -123,3 +123,13 @@ def attend(kc, vc, table, lens, starts, q, heads, rope, scale=None, window=0, ou
                     b = b + (out[first + j, h].abs() + b) * U[torch.bfloat16]
                 bound[first + j, h] = b + 1e-30
     return out.reshape(tokens, -1), bound.reshape(tokens, -1), mine
+
+
+def rows_off(got, want, dim, skip=None):
+    """How far each (token, head) row is off, relative to its length; element `skip` left out.  The bound above adds up what all
+    roundings could do together, which for a bf16 result over many keys is more than the result: whole key tiles could be missing
+    inside it.  The roundings are independent (result, weights and q: each at most 2^-8 of its terms, 2^-8 / sqrt(3) in the mean
+    square), together at most 2^-8 of a row of values around 0; a test allows 2^-7."""
+    keep = [i for i in range(dim) if i != skip]
+    d, w = ((x.double().cpu().reshape(-1, dim)[:, keep]) for x in (got - want, want))
+    return d.norm(dim=1) / w.norm(dim=1).clamp(min=1e-12)

@@ -382,6 +382,27 @@ def test_what_is_not_finite_reaches_only_the_tokens_that_see_it(F, ctx, out_dtyp
         assert fine[sees][:, 2:][..., keep].all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("lens,new,heads", [([2600], [57], 5), ([2600, 1900], [90, 30], 4), ([130, 150], [90, 100], 4), ([900], [6], 2)])
+def test_rows_of_a_block_done_again_hold_every_key(F, ctx, dtype, dim, bad, lens, new, heads):
+    """A value that is not finite, seen by the last rows only: the block is evaluated again key by key, on a long cache by several
+    CTAs.  Every row that does not see it, and the rest of the rows that do, to the limit on rows."""
+    b = Batch(F, ctx, lens=lens, new=new, heads=heads, kv_heads=1, dim=dim, page=32, dtype=dtype, base=1e6)
+    want, _, _ = R.attend(b.cache.k, b.cache.v, b.table, b.lens, b.starts, b.q, heads, b.rope_ref, out_dtype=BF)
+    sees = []
+    for i, (n, m) in enumerate(zip(lens, new)):
+        at = n - 1 - m // 3
+        b.cache.v[int(b.table[i, at // 32]), 0, at % 32, 7] = bad
+        sees += [n - m + j >= at for j in range(m)]
+    sees = torch.tensor(sees)[:, None].expand(-1, heads).reshape(-1)
+    y = b.cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=BF).double().cpu()
+    assert not torch.isfinite(y.reshape(-1, dim)[sees, 7]).any()
+    assert R.rows_off(y, want, dim)[~sees].max() <= 2.0 ** -7
+    assert R.rows_off(y, want, dim, skip=7)[sees].max() <= 2.0 ** -7
+
+
 @pytest.mark.parametrize("out_dtype", [torch.float32, BF])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("dim", [64, 128, 256])
@@ -726,6 +747,27 @@ def test_a_cache_past_32_bit_offsets(F, ctx):
         y = cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=ty).double().cpu()
         want, bound, _ = R.attend(kc, vc, small, lens, b.starts, b.q, 8, b.rope_ref, out_dtype=ty)
         assert ((y - want).abs() <= bound).all()
+
+
+def test_rows_of_a_cache_past_32_bit_offsets(F, ctx):
+    """The same with enough new tokens on enough keys for the prompt kernel, to the limit on rows."""
+    n_pages = (1 << 31) // (8 * 64 * 128) + 24
+    cache = F.KVCache.empty(ctx, n_pages, 64, 8, 128)
+    lens = [600, 400]
+    table = torch.full((2, 10), -1, dtype=torch.int32)
+    table[0] = torch.tensor([n_pages - 1 - 2 * i if i % 2 else i for i in range(10)])
+    table[1, :7] = torch.tensor([n_pages - 2 - 2 * i if i % 2 == 0 else 100 + i for i in range(7)])
+    b = Batch(F, ctx, lens=lens, new=lens, heads=8, kv_heads=8, page=64, fill=False)
+    b.seqs = F.KVSeqs(table.cuda(), b.seqs.lens, b.seqs.starts)
+    cache.append(b.seqs, b.k, b.v, rope=b.rope)
+    ids = sorted(set(int(x) for x in table.flatten() if x >= 0))
+    small = torch.full_like(table, -1)
+    for i, p in enumerate(ids):
+        small[table == p] = i
+    kc, vc = cache.k[ids], cache.v[ids]
+    y = cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=BF).double().cpu()
+    want, _, _ = R.attend(kc, vc, small, lens, b.starts, b.q, 8, b.rope_ref, out_dtype=BF)
+    assert R.rows_off(y, want, 128).max() <= 2.0 ** -7
 
 
 # ---- the decoder stack with attention -----------------------------------------------------------------------

@@ -333,6 +333,28 @@ def test_a_scale_that_is_0_in_32_bits_is_refused(on_gpu):
     assert ctx.calls[0][1][8] == 1e-44 and ctx.calls[1][1][8] == 0.0
 
 
+def test_the_limit_on_rows_sees_missing_keys():
+    """A page of 32 keys out of 2600 lies far inside the elementwise bound of a bf16 result, and outside the limit on rows."""
+    import torch
+
+    import kv_ref as R
+    g = torch.Generator().manual_seed(2)
+    kc, vc = (torch.randn((82, 1, 32, 128), generator=g).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn((12, 2 * 128), generator=g)
+    table = torch.randperm(82, generator=g)[None].int()
+    want, bound, _ = R.attend(kc, vc, table, [2600], [0, 12], q, 2, dict(rotary=0), out_dtype=torch.bfloat16)
+    rounded = want.bfloat16().double()
+    assert R.rows_off(rounded, want, 128).max() <= 2.0 ** -8
+    for gone in (0, 40, 80):
+        less = table.clone()
+        less[0, gone] = -1
+        got, _, _ = R.attend(kc, vc, less, [2600], [0, 12], q, 2, dict(rotary=0), out_dtype=torch.bfloat16)
+        assert ((got - want).abs() <= bound).all() and R.rows_off(got, want, 128).min() > 2.0 ** -7
+    spoilt = want.clone()
+    spoilt[3, 5] = float("inf")
+    assert R.rows_off(spoilt, want, 128, skip=5).max() == 0 and not torch.isfinite(R.rows_off(spoilt, want, 128)[6])
+
+
 def test_the_64_bit_evaluation_against_differences():
     """The tests' own reference: rotation keeps lengths and composes, attention is the weighted mean of its definition."""
     import torch
