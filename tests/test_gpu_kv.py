@@ -717,6 +717,22 @@ def test_no_tokens_and_no_sequences(F, ctx):
     assert b.cache.attend(s, b.q).shape[0] == 0
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+def test_caches_and_tables_without_pages(F, ctx, dim, out_dtype):
+    """Nothing to append to and nothing to see: zeros, whatever the lengths say."""
+    b = Batch(F, ctx, lens=[30, 200, 1], new=[30, 100, 1], heads=4, kv_heads=2, dim=dim, pad_rows=1)
+    none = F.KVCache(ctx, b.cache.k[:0], b.cache.v[:0])
+    bare = F.KVSeqs(b.seqs.page_table[:, :0], b.seqs.lens, b.seqs.starts)
+    k0 = b.cache.k.clone()
+    for c, s in ((none, b.seqs), (b.cache, bare), (none, bare)):
+        c.append(s, b.k, b.v, rope=b.rope)
+        y = c.attend(s, b.q, rope=b.rope, out=torch.full((132, 4 * dim), 7.0, dtype=out_dtype, device="cuda"))
+        assert (y[:131] == 0).all() and (y[131] == 7).all()
+    assert torch.equal(b.cache.k.view(torch.int16), k0.view(torch.int16))
+    b.check_attend(out_dtype=out_dtype)
+
+
 def test_starts_that_make_no_sense_stay_inside_the_activations(F, ctx):
     b = Batch(F, ctx, lens=[40, 40, 40], new=[10, 10, 10])
     for starts in ([0, 50, 20, 30], [-9, 10, 2 ** 31 - 1, 5], [30, 20, 10, 0], [5, 5, 5, 5]):
