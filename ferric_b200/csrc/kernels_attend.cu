@@ -16,16 +16,18 @@ int* gemm_status_word();   // device address of the status word shared with the 
 // ---------------------------------------------------------------------------------------------------------------------
 // attend_split_kernel: few query rows against many keys, kept to f32 accuracy.
 //
-// 64 sequences over 0.7k-8k keys (40 over 8 heads x 128, f16): 190 us = 6.2 TB/s; one over 131000 (bf16): 116-123 us = 4.4-4.6
-// TB/s, of which the stream itself takes about 80.  Bound by the cache's bytes from HBM (2 * 2 * head_dim per key and head; at 5 query heads per key-value head that is 5
-// multiply-adds per byte).  So: one CTA reads a tile of 64 keys once for all query heads of its key-value head, tiles travel
+// 64 sequences over 0.7k-8k keys (40 over 8 heads x 128, f16): 196 us a call = 6.1 TB/s (190 in a captured graph); on a bf16 cache
+// 229 in a graph: three parts of q and the sums pass the 168 registers that two CTAs per SM leave, and spill (308 bytes stored, 636
+// loaded).  One over 131000 (bf16): 116 us = 4.6 TB/s, of which the stream itself takes about 80.  Bound by the cache's bytes from
+// HBM (2 * 2 * head_dim per key and head; at 5 query heads per key-value head that is 5 multiply-adds per byte).  So: one CTA
+// reads a tile of 64 keys once for all query heads of its key-value head, tiles travel
 // by TMA into a ring filled by a warp of its own, and the line of all tiles is cut evenly over the resident CTAs
 // (kv_index.h); a block that several CTAs share leaves pieces (m, l, unnormalised output) in the workspace, which the CTA
 // that finishes last joins, in piece order whoever that is, so the same call gives the same bits.
 //
 // The products run on mma.sync m16n8k16: decode has 1 to 8 query rows per key-value head, and its 16-row operand has room
 // for the q of 8 rows twice.  The cache's elements are 16-bit already; q and the weights p are f32, and rounding them to 16
-// bits would put 2^-9 of error where the o product takes f32 -- so they are split into 16-bit parts that add up to (almost)
+// bits would put up to 2^-8 of error where the o product takes f32 -- so they are split into 16-bit parts that add up to (almost)
 // the f32 value: two f16 parts (22 bits), the first in rows 0-7 and the second in rows 8-15 of one MMA, or three bf16 parts
 // (24 bits), the third in a second MMA.  A row's two halves meet in one thread's registers (rows g and g + 8).  f16 parts
 // are scaled away from f16's lower end first: q by a power of two per row, p by 2^14.

@@ -1,6 +1,7 @@
 // attend_prompt_kernel: attention of many new tokens (prompts and chunks of them), result in bf16, on tcgen05.
 //
-// A prompt of 4096 (40 over 8 heads x 128): 271 us = 635 TFLOP/s in bf16; chunks of three prompts in f16: 202 us = 937 TFLOP/s.
+// A prompt of 4096 (40 over 8 heads x 128, bf16): 285 us a call = 603 TFLOP/s (267 in a captured graph); chunks of three prompts
+// (f16): 225 us = 841 TFLOP/s (208).  At head_dim 256 a prompt of 4096 (16 over 4 heads) takes 254 us in bf16, 202 in f16 (graph).
 // Bound by the tensor cores (4 head_dim flop per visible pair and query head), short of it by a block's set-up and end and, in
 // bf16, by a ring of three stages.  A CTA takes 256 query rows (head_dim 256:
 // 128) of one key-value head -- (token, query head of the group) pairs, so that all heads of the group share the keys it
@@ -13,10 +14,10 @@
 // The maximum of a row only has to keep 2^(s - m) in range, so it moves -- and O is rescaled, a round trip through registers
 // -- only when the new one exceeds the old one by more than 2^kSlack; the division by the sum makes up for the rest.
 //
-// Rounding: the weights are rounded once to the cache's type (they multiply its values on the tensor cores; 2^-9 of a
-// weight in bf16, as much as the result's own rounding), summed in f32 before that.  q is rounded to f16 for an f16 cache, each
+// Rounding: the weights are rounded once to the cache's type (they multiply its values on the tensor cores; up to 2^-8 of
+// a weight in bf16, as much as the result's own rounding), summed in f32 before that.  q is rounded to f16 for an f16 cache, each
 // row scaled by a power of two first (undone on its scores, in the subtraction of the maximum); for a bf16 cache it is split into
-// two bf16 parts, since one alone would move every score by up to 2^-9 of its terms.
+// two bf16 parts, since one alone would move every score by up to 2^-8 of its terms.
 #include <string.h>
 
 #include <type_traits>
@@ -741,9 +742,16 @@ int32_t launch_prompt(cudaStream_t st, const KvCacheView& c, const KvSeqsView& s
 }
 }  // namespace
 
-// Above 32 query rows a sequence and key-value head the tensor cores' tiles of 128 rows win although most of one is empty
-// (8 sequences x 2000 keys, 40 over 8 heads x 128 in bf16: 35 rows 57 us against the split kernel's 86; 65 rows 56 against
-// 138); where a result is wanted in f32, the split kernel runs.
+// Above 32 query rows a sequence and key-value head the tensor cores' tiles of 128 rows win, or cost little, although most of one is
+// empty; where a result is wanted in f32, the split kernel runs.  Measured in a graph, this kernel / the split kernel, us:
+//                                       8 sequences x 2000 keys            48 sequences x 2000 keys
+//   40 over 8 heads x 128, bf16    30 rows 54 / 57    40 rows 54 / 85     30: 185 / 209   40: 186 / 375
+//   40 over 8 heads x 128, f16             50 / 39             50 / 56         162 / 119        162 / 213
+//   16 over 2 heads x 256, bf16    32 rows 51 / 65    40 rows 51 / 61     32:  70 / 130   40:  70 / 210
+//   16 over 2 heads x 256, f16             49 / 52             49 / 45          53 /  84         54 / 136
+//   32 over 8 heads x 64, bf16     32 rows 36 / 30    40 rows 36 / 41     32: 141 /  94   40: 141 / 163
+//   32 over 8 heads x 64, f16              35 / 25             35 / 33         132 /  65        132 / 113
+// The rows are the batch's average, so what runs for a sequence, and how its weights are rounded, depends on the others.
 bool attend_prompt_eligible(const KvCacheView& c, const KvSeqsView& s, const AttendArgs& a)
 {
     return a.out_bf16 && ((long long)s.tokens + s.seqs - 1) / s.seqs * (a.heads / c.heads) > 32;

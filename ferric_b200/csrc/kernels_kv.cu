@@ -9,8 +9,8 @@ namespace ferric {
 // and one chain of loads (lengths -> page) for few.  A thread takes 16 elements of HP heads, k and v: a rotated unit is eight
 // pairs -- two runs of eight elements half the rotated width apart, or one run of sixteen for adjacent pairs -- so reads are
 // float4, writes are 16 bytes, and the unit's eight angles serve all of its heads.  The rows are requested before the
-// lengths and pages are looked up: nothing about where they go decides what is read.  16384 tokens x 8 heads x 128: 36-37 us =
-// 5.4-5.6 TB/s; one token 2.0 us.  A token row outside every sequence,
+// lengths and pages are looked up: nothing about where they go decides what is read.  16384 tokens x 8 heads x 128: 36 us =
+// 5.6 TB/s; one token 2.3 us on the device.  A token row outside every sequence,
 // or a position without a page, writes nothing.
 template <typename T, int HP>
 __global__ void __launch_bounds__(256) kv_append_kernel(KvCacheView c, KvSeqsView s, RopeView r, const float* __restrict__ k, size_t ldk,

@@ -636,8 +636,8 @@ class KVCache:
                out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """Attention of the new tokens over what the cache holds (``ferric_cuda_kv_attend``): q [tokens, heads * head_dim],
         rotated by ``rope``; each token sees its sequence's keys up to its own position, the last ``window`` of them where
-        that is set.  Returns [tokens, heads * head_dim] in ``out_dtype`` (float32, or bfloat16 for the prefill products),
-        or fills ``out``; rows of no sequence are left as they were (in a result made here: as the memory was)."""
+        that is set.  Returns [tokens, heads * head_dim] in ``out_dtype`` (float32, kept to f32 accuracy, or bfloat16 for the
+        prefill products, where long batches round the weights to 16 bits too), or fills ``out``; rows of no sequence are left as they were (in a result made here: as the memory was)."""
         q, n, cols, pq, ldq = self._rows(q, "q")
         if cols % self.head_dim:
             raise ValueError(f"q has {cols} columns, heads have {self.head_dim}")

@@ -376,10 +376,14 @@ int32_t ferric_cuda_kv_append(ferric_cuda_ctx *ctx, const ferric_kv_cache *cache
  * sequence at positions <= its own, the last `window` of them where window > 0 -- query head h reading key-value head
  * h / (n_q_heads / cache heads).  q is f32 like k above (rotated here: `rope` as for append); scale 0 = 1 / sqrt(head_dim).
  * out is FERRIC_GGML_F32 (the decode products' activation type: the whole product is then kept to f32 accuracy) or
- * FERRIC_GGML_BF16 (the prefill products'), 16-byte aligned with row stride ldo (0 = dense; a multiple of 16 bytes), and
- * must not overlap q (refused).  A token that sees no key gets zeros; output rows outside every sequence are left as they were.  The
- * new tokens' own keys must have been appended.  A key or value element that is not finite reaches only the tokens that see it;
- * a key with a score of -inf weighs nothing (such infinities come of an append to f16 of numbers above 65504).
+ * FERRIC_GGML_BF16 (the prefill products').  A bf16 result above 32 query rows per sequence and key-value head, on the batch's
+ * average, has the weights rounded to the cache's type as well, and q to f16 (f16 cache) or to two bf16 parts: on a bf16 cache
+ * it is off by 2.1e-3 of a row's length, where rounding the result alone is 1.6e-3, on an f16 cache by no more than that alone.
+ * Which of the two a sequence gets depends on its batch.  q and scale may be of any size as long as scale * q fits f32.
+ * out is 16-byte aligned with row stride ldo (0 = dense; a multiple of 16 bytes), and must not overlap q (refused).  A token that
+ * sees no key gets zeros; output rows outside every sequence are left as they were.  The new tokens' own keys must have been
+ * appended.  A key or value element that is not finite reaches only the tokens that see it; a key with a score of -inf weighs
+ * nothing (such infinities come of an append to f16 of numbers above 65504; a token with no other key gets zeros).
  * Calls on one context share a workspace (ferric_cuda_attend_reserve, allocated by the first call otherwise, which must then
  * not be under capture): graphs captured on one context must not be replayed at the same time, nor beside its other calls
  * -- give each stream of replays a context of its own.  Waits inside the kernels are bounded; ferric_cuda_gemm_status reports one that ran out. */
