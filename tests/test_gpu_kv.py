@@ -426,6 +426,27 @@ def test_an_infinite_key_with_a_score_of_minus_infinity_weighs_nothing(F, ctx, o
     b.check_rows(y, want, mine, out_dtype)
 
 
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens,new", [([200, 70, 9, 40], None), ([200, 300], [5, 3]), ([2600], [57])])
+def test_a_query_that_is_not_finite_stays_in_its_row(F, ctx, out_dtype, dtype, dim, lens, new):
+    b = Batch(F, ctx, lens=lens, new=new, heads=4, kv_heads=1, dim=dim, page=32, dtype=dtype)
+    want, bound, mine = R.attend(b.cache.k, b.cache.v, b.table, b.lens, b.starts, b.q, 4, b.rope_ref, out_dtype=out_dtype)
+    b.q[0, 3] = float("nan")
+    b.q[1, dim + 2] = float("inf")
+    b.q[b.tokens - 1, 2 * dim:3 * dim] = float("-inf")
+    y = b.cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=out_dtype).double().cpu()
+    hit = torch.zeros((b.tokens, 4), dtype=torch.bool)
+    hit[0, 0] = hit[1, 1] = hit[b.tokens - 1, 2] = True
+    at = hit.reshape(-1)
+    assert torch.isnan(y.reshape(-1, dim)[at]).all()
+    fine = ((y - want).abs() <= bound).reshape(-1, dim)
+    assert fine[~at].all()
+    if out_dtype == BF:
+        assert R.rows_off(y, want, dim)[~at].max() <= 2.0 ** -7
+
+
 def test_value_outside_the_window_does_not_leak(F, ctx):
     b = Batch(F, ctx, lens=[200, 200], new=[1, 40], heads=4, kv_heads=1, page=16)
     for i in range(2):
