@@ -17,7 +17,7 @@ int* gemm_status_word();   // device address of the status word shared with the 
 // attend_split_kernel: few query rows against many keys, kept to f32 accuracy.
 //
 // 64 sequences over 0.7k-8k keys (40 over 8 heads x 128, f16): 196 us a call = 6.1 TB/s (190 in a captured graph); on a bf16 cache
-// 229 in a graph: three parts of q and the sums pass the 168 registers that two CTAs per SM leave, and spill (308 bytes stored, 636
+// 229 in a graph: three parts of q and the sums pass the 168 registers that two CTAs per SM leave, and spill (288 bytes stored, 624
 // loaded).  One over 131000 (bf16): 116 us = 4.6 TB/s, of which the stream itself takes about 80.  Bound by the cache's bytes from
 // HBM (2 * 2 * head_dim per key and head; at 5 query heads per key-value head that is 5 multiply-adds per byte).  So: one CTA
 // reads a tile of 64 keys once for all query heads of its key-value head, tiles travel
@@ -75,15 +75,24 @@ struct SplitBars {
     unsigned valid[8];           // per stage: which of the tile's pages exist
     long long warp_sum[16];
     long long item_start;
-    int seq, tainted, last;
+    int seq, last;
+    int tainted;                 // bit 0: a value that is not finite; bit 1: weights that are NaN (bf16)
+    int inf_count, inf_key[32];  // infinite keys
     volatile int abort;          // a wait ran out
 };
+static_assert(sizeof(SplitBars) <= 512, "SplitCfg::kFixed has 512 bytes for it");
 
 __device__ __forceinline__ float ex2f(float x)
 {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// hi + lo, where an infinite or NaN lo does not count: the first part of q decides on an infinite key.
+__device__ __forceinline__ float add_finite(float hi, float lo)
+{
+    asm("min.xorsign.abs.f32 %0, %0, %1;" : "+f"(lo) : "f"(3.4028235e38f));
+    return hi + lo;
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
 {
@@ -159,7 +168,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         }
         mbar_init(&bar->q_full, 1);
         mbar_init(&bar->q_empty, C::kWarps);
-        bar->tainted = bar->abort = 0;
+        bar->tainted = bar->abort = bar->inf_count = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_launch_dependents();
@@ -435,7 +444,8 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             for (int i = 0; i < C::kKeys / 8; i++) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float v = sc[i][e] + sc[i][e + 2];
+                    // (in bf16 the zeros beside the third part have been multiplied by the key too)
+                    float v = BF ? sc[i][e] + sc[i][e + 2] : add_finite(sc[i][e], sc[i][e + 2]);
                     if (!BF) v *= unscale;
                     if (MASKED) {
                         const int key = key0 + 8 * i + e;
@@ -494,7 +504,7 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                         mma_kv<BF>(o[2 * np + 1], 0u, E[0], 0u, E[1], vf[2], vf[3]);
                     }
                 }
-                if (MASKED && odd && b.j0 != b.j1) bar->tainted = 1;
+                if (MASKED && odd && b.j0 != b.j1) atomicOr(&bar->tainted, 1);
             }
         };
 
@@ -515,16 +525,14 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         // the row's halves and the quad's sums together
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        // An infinite key: the score of q in parts is inf - inf or 0 inf where that of q itself may be -inf, a weight of 0.  The sum of
-        // the weights shows it, and such a block is done again too.
-        if (l != l && my_r < b.rows) bar->tainted = 1;
+        if (BF && l != l && my_r < b.rows) atomicOr(&bar->tainted, 2);
         float2 oo[NT];
 #pragma unroll
         for (int i = 0; i < NT; i++) oo[i] = make_float2(o[i][0] + o[i][2], o[i][1] + o[i][3]);
 
         // the warps that share rows: pairwise through `buf`, in a fixed order
         named_bar_sync(1, kCons);
-        const bool tainted = bar->tainted != 0;
+        const int tainted = bar->tainted;
         auto give = [&](float* slot) {
 #pragma unroll
             for (int i = 0; i < NT; i++) *reinterpret_cast<float2*>(slot + i * 64 + lane * 2) = oo[i];
@@ -564,31 +572,44 @@ attend_split_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 
         // now the kn == 0 warps hold their tile's rows: lane (g, t) elements 8 i + 2 t + {0, 1} of row g
         if (tainted) {
-            // A value that some rows of the block see and others do not is not finite -- weight 0 does not hide it in a matrix
-            // product -- or a row's weights are NaN.  The rows again, one by one and key by key, over this CTA's tiles of the block.
+            // A value that some rows of the block see and others do not is not finite: weight 0 does not hide it in a matrix
+            // product.  The rows again, one by one and key by key, over this CTA's tiles of the block.  Or weights are NaN: the rows
+            // that infinite keys spoilt, if there are any.
+            if (tainted == 2)
+                list_infinite_keys<T, D>(c, s, seq, head, kv_max(b.lo, (b.t0 + ta) * kAttendTile), kv_min(b.hi, (b.t0 + tb) * kAttendTile), warp,
+                                         C::kWarps, lane, &bar->inf_count, bar->inf_key, 32);
             named_bar_sync(1, kCons);
-            for (int r = warp; r < b.rows; r += C::kWarps) {
-                float* q = buf + r * C::kPitch;   // the row's q, then its results
-                const int j = token_of(r), h = head * group + head_of(r), pos = span.pos(j);
-                const float* src = a.q + (size_t)(span.first + j) * a.ldq + (size_t)h * D;
-                __syncwarp();
-                for (int e = lane; e < D; e += 32) q[e] = rope_element(rope, src, e, pos) * (a.scale * kLog2e);
-                __syncwarp();
-                float pm, pl, acc[D / 32];
-                attend_row_plain<T, D>(c, s, seq, head, q, kv_max(kv_seen_lo(pos, a.window), (b.t0 + ta) * kAttendTile),
-                                       kv_min(kv_seen_hi(c, s, pos), (b.t0 + tb) * kAttendTile), lane, &pm, &pl, acc);
-                __syncwarp();
+            const int infs = bar->inf_count;
+            if ((tainted & 1) || infs > 0) {
+                for (int r = warp; r < b.rows; r += C::kWarps) {
+                    float* q = buf + r * C::kPitch;   // the row's q, then its results
+                    const int j = token_of(r), h = head * group + head_of(r), pos = span.pos(j);
+                    const int lo = kv_seen_lo(pos, a.window), hi = kv_seen_hi(c, s, pos);
+                    const float* src = a.q + (size_t)(span.first + j) * a.ldq + (size_t)h * D;
+                    __syncwarp();
+                    for (int e = lane; e < D; e += 32) q[e] = rope_element(rope, src, e, pos) * (a.scale * kLog2e);
+                    __syncwarp();
+                    const bool again = (tainted & 1) || infinite_keys_weigh_nothing<T, D>(c, s, seq, head, q, lo, hi, infs, bar->inf_key, lane);
+                    if (lane == 0) q[D + 2] = again ? 1.0f : 0.0f;
+                    if (!again) continue;
+                    float pm, pl, acc[D / 32];
+                    attend_row_plain<T, D>(c, s, seq, head, q, kv_max(lo, (b.t0 + ta) * kAttendTile), kv_min(hi, (b.t0 + tb) * kAttendTile), lane, &pm,
+                                           &pl, acc);
+                    __syncwarp();
 #pragma unroll
-                for (int e = 0; e < D / 32; e++) q[lane + 32 * e] = acc[e];
-                if (lane == 0) *reinterpret_cast<float2*>(q + D) = make_float2(pm, pl);
+                    for (int e = 0; e < D / 32; e++) q[lane + 32 * e] = acc[e];
+                    if (lane == 0) *reinterpret_cast<float2*>(q + D) = make_float2(pm, pl);
+                }
             }
             named_bar_sync(1, kCons);
-            if (tid == 0) bar->tainted = 0;
+            if (tid == 0) bar->tainted = bar->inf_count = 0;
             const float* row = buf + (wm * 8 + g) * C::kPitch;
+            if (((tainted & 1) || infs > 0) && my_r < b.rows && row[D + 2] != 0.0f) {
 #pragma unroll
-            for (int i = 0; i < NT; i++) oo[i] = *reinterpret_cast<const float2*>(row + 8 * i + 2 * t4);
-            m = row[D];
-            l = row[D + 1];
+                for (int i = 0; i < NT; i++) oo[i] = *reinterpret_cast<const float2*>(row + 8 * i + 2 * t4);
+                m = row[D];
+                l = row[D + 1];
+            }
         }
 
         auto out_at = [&](int r, int e) {   // element e of row r of the block

@@ -34,8 +34,9 @@ struct PromptBars {
     uint64_t full[8], empty[8];
     uint64_t s_full[2], p_full[2], pv_done[2], turn[2];
     uint32_t tmem;
-    int tainted, last;
+    int tainted, last;    // tainted: bit 0 a value that is not finite, bit 1 weights that are NaN
     volatile int abort;   // a wait ran out
+    int inf_count, inf_key[32];
 };
 template <typename T, int D>
 struct PromptCfg {
@@ -257,7 +258,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             mbar_init(&bar->pv_done[i], 1);
             mbar_init(&bar->turn[i], 1);
         }
-        bar->tainted = bar->abort = 0;
+        bar->tainted = bar->abort = bar->inf_count = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // Q: rotated, scaled to log2 units, in 16-bit parts, K-major with a 128-byte swizzle.  A thread takes one token's 16
@@ -392,7 +393,7 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                     auto bad = [&](uint32_t v) { return (v & e) == e || (v & (e << 16)) == (e << 16); };
                     if (k0 + row >= b.lo && k0 + row < b.hi) odd |= bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
                 }
-                if (odd) bar->tainted = 1;
+                if (odd) atomicOr(&bar->tainted, 1);
                 __syncwarp();
             }
         }
@@ -578,8 +579,8 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
         wait(&bar->pv_done[x], PRE == 2 ? (tiles - 1) & 1 : 0, 57);
         tc_fence_after();
-        // an infinite key: q's parts (or an element rounded to 0) make inf - inf or 0 inf of what may be a score of -inf
-        if (have && l != l) bar->tainted = 1;
+        // an infinite key: q's parts (or an element rounded to 0) make inf - inf or 0 inf of what may be a score of -inf (see below)
+        if (have && l != l) atomicOr(&bar->tainted, 2);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         // The result goes through the tile's place of Q, done with since its last S: written row by row as tensor memory
         // holds it (16-byte chunks, permuted so that eight rows do not meet in a bank), stored row-contiguously.
@@ -633,7 +634,14 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     }
     if (warp == C::kSoftWarps)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
-    if (bar->tainted) {
+    const int tainted = bar->tainted;
+    if (tainted == 2) {   // NaN is right, unless infinite keys made it where their scores are -inf
+        list_infinite_keys<T, D>(c, s, seq, head, kv_max(b.lo, t0 * KT), kv_min(b.hi, (t0 + tiles) * KT), warp, C::kThreads / 32, lane, &bar->inf_count,
+                                 bar->inf_key, 32);
+        __syncthreads();
+    }
+    const int infs = bar->inf_count;
+    if ((tainted & 1) || infs > 0) {
         // the rows one by one, key by key (what was stored above is overwritten)
         float* q = reinterpret_cast<float*>(qs) + warp * D;
         for (int row = warp; row < b.rows; row += C::kThreads / 32) {
@@ -642,9 +650,10 @@ attend_prompt_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             __syncwarp();
             for (int e = lane; e < D; e += 32) q[e] = rope_element(rope, src, e, pos) * (a.scale * kLog2e);
             __syncwarp();
+            const int lo = kv_seen_lo(pos, a.window), hi = kv_seen_hi(c, s, pos);
+            if (!(tainted & 1) && !infinite_keys_weigh_nothing<T, D>(c, s, seq, head, q, lo, hi, infs, bar->inf_key, lane)) continue;
             float m, l, acc[D / 32];
-            attend_row_plain<T, D>(c, s, seq, head, q, kv_max(kv_seen_lo(pos, a.window), t0 * KT), kv_min(kv_seen_hi(c, s, pos), (t0 + tiles) * KT), lane,
-                                   &m, &l, acc);
+            attend_row_plain<T, D>(c, s, seq, head, q, kv_max(lo, t0 * KT), kv_min(hi, (t0 + tiles) * KT), lane, &m, &l, acc);
             if (parts > 1) {
 #pragma unroll
                 for (int e = 0; e < D / 32; e++) {

@@ -121,4 +121,56 @@ __device__ __forceinline__ void attend_row_plain(const KvCacheView& c, const KvS
     *l_out = l;
 }
 
+// An infinite key makes inf - inf or 0 inf of q in parts where the score of q itself may be -inf, a weight of 0.  Kernels that see it
+// only by a row's weights being NaN look for such keys then, and evaluate again the rows whose scores it spoilt; a NaN key, or one
+// with a score of +inf, has NaN for its result as it is.
+//
+// Keys in [lo, hi) of one sequence and head that hold an infinity: this warp's share (`warps` warps in all) is counted in *n and the
+// first `cap` of all are listed.
+template <typename T, int D>
+__device__ __forceinline__ void list_infinite_keys(const KvCacheView& c, const KvSeqsView& s, int seq, int h, int lo, int hi, int warp, int warps,
+                                                   int lane, int* n, int* list, int cap)
+{
+    constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;   // of a key; keys a warp reads at once
+    constexpr unsigned kAll = kLanes == 32 ? 0xffffffffu : (1u << (kLanes & 31)) - 1u;
+    const T* K = reinterpret_cast<const T*>(c.k);
+    for (int k0 = lo + warp * kAtOnce; k0 < hi; k0 += warps * kAtOnce) {
+        const int key = k0 + lane / kLanes;
+        const long long off = key < hi ? kv_offset(c, s, seq, h, key) : -1;
+        bool found = false;
+        if (off >= 0) {
+            const uint4 w = *reinterpret_cast<const uint4*>(K + off + lane % kLanes * 8);
+            const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) found |= fabsf(kv_to_float(e[i])) == INFINITY;
+        }
+        const unsigned any = __ballot_sync(0xffffffffu, found);
+        if (lane % kLanes == 0 && ((any >> lane) & kAll)) {
+            const int at = atomicAdd(n, 1);
+            if (at < cap) list[at] = key;
+        }
+    }
+}
+
+// Whether a row of NaN weights, with its `q` (as for attend_row_plain) in shared memory, is to be evaluated again: it sees one of the
+// `n` infinite keys (of which 32 are listed), and every one that it sees has a score of -inf.  Otherwise NaN is its result.
+template <typename T, int D>
+__device__ __forceinline__ bool infinite_keys_weigh_nothing(const KvCacheView& c, const KvSeqsView& s, int seq, int h, const float* q, int lo, int hi,
+                                                            int n, const int* list, int lane)
+{
+    bool sees = n > 32;
+    for (int i = 0; i < kv_min(n, 32); i++) {
+        const int key = list[i];
+        if (key < lo || key >= hi) continue;
+        const T* k = reinterpret_cast<const T*>(c.k) + kv_offset(c, s, seq, h, key);
+        float dot = 0.0f;
+        for (int e = lane; e < D; e += 32) dot = fmaf(q[e], kv_to_float(k[e]), dot);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (!(dot == -INFINITY)) return false;
+        sees = true;
+    }
+    return sees;
+}
+
 }  // namespace ferric

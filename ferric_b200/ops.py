@@ -514,8 +514,9 @@ def _pitch(t: torch.Tensor, name: str) -> int:
 
 class KVSeqs:
     """The batch a cache call works on (``ferric_kv_seqs``), int32 CUDA tensors read when the kernels run: ``page_table``
-    [n_seqs, max_pages], each sequence with a row of its own (rows may name the same pages); ``lens`` [n_seqs], each sequence's length with its new tokens; ``starts`` [n_seqs + 1], the first
-    activation row of each sequence, or None when row i is the one new token of sequence i."""
+    [n_seqs, max_pages], each sequence with a row of its own (rows may name the same pages); ``lens`` [n_seqs], each sequence's
+    length with its new tokens; ``starts`` [n_seqs + 1], the first activation row of each sequence, or None when row i is the one
+    new token of sequence i."""
 
     def __init__(self, page_table: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None):
         for name, t, dim in (("page_table", page_table, 2), ("lens", lens, 1), ("starts", starts, 1)):
@@ -637,7 +638,8 @@ class KVCache:
         """Attention of the new tokens over what the cache holds (``ferric_cuda_kv_attend``): q [tokens, heads * head_dim],
         rotated by ``rope``; each token sees its sequence's keys up to its own position, the last ``window`` of them where
         that is set.  Returns [tokens, heads * head_dim] in ``out_dtype`` (float32, kept to f32 accuracy, or bfloat16 for the
-        prefill products, where long batches round the weights to 16 bits too), or fills ``out``; rows of no sequence are left as they were (in a result made here: as the memory was)."""
+        prefill products, where long batches round the weights to 16 bits too), or fills ``out``; rows of no sequence are left as
+        they were (in a result made here: as the memory was)."""
         q, n, cols, pq, ldq = self._rows(q, "q")
         if cols % self.head_dim:
             raise ValueError(f"q has {cols} columns, heads have {self.head_dim}")

@@ -429,6 +429,34 @@ def test_an_infinite_key_with_a_score_of_minus_infinity_weighs_nothing(F, ctx, o
 @pytest.mark.parametrize("out_dtype", [torch.float32, BF])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens,new", [([200, 70, 9, 40], None), ([200, 300], [5, 3]), ([300, 150], [140, 150]), ([2600], [57])])
+def test_nan_and_infinite_keys_together(F, ctx, out_dtype, dtype, dim, lens, new):
+    """Keys with NaN in the first sequence, infinities with a score of -inf in all, both in the last: every token that sees a NaN key is
+    NaN, every other is as if the infinite keys were not there."""
+    b = Batch(F, ctx, lens=lens, new=new, heads=5, kv_heads=1, dim=dim, page=16, dtype=dtype, rotary=0)
+    b.q[:, 5::dim] = -b.q[:, 5::dim].abs() - 0.1
+    there = b.table.clone()
+    nan_at = {0: lens[0] - 3, len(lens) - 1: lens[-1] - 2}
+    rows, t = [], 0
+    for i, (n, m) in enumerate(zip(lens, b.new)):
+        if n > 40:
+            b.cache.k[int(there[i, 1]), 0, :, 5] = float("inf")
+            b.table[i, 1] = -1
+        if i in nan_at:
+            b.cache.k[int(there[i, nan_at[i] // 16]), 0, nan_at[i] % 16, 9] = float("nan")
+        rows += [i in nan_at and n - m + j >= nan_at[i] for j in range(m)]
+    sees = torch.tensor(rows)
+    y = b.cache.attend(b.seqs, b.q, rope=b.rope, out_dtype=out_dtype).double().cpu()
+    want, bound, _ = R.attend(b.cache.k, b.cache.v, b.table, b.lens, b.starts, b.q, b.heads, b.rope_ref, out_dtype=out_dtype)
+    assert sees.any() and torch.isnan(y[sees]).all()
+    assert ((y - want).abs() <= bound)[~sees].all()
+    if out_dtype == BF and not sees.all():
+        assert R.rows_off(y[~sees], want[~sees], dim).max() <= 2.0 ** -7
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("lens,new", [([200, 70, 9, 40], None), ([200, 300], [5, 3]), ([2600], [57])])
 def test_a_query_that_is_not_finite_stays_in_its_row(F, ctx, out_dtype, dtype, dim, lens, new):
     b = Batch(F, ctx, lens=lens, new=new, heads=4, kv_heads=1, dim=dim, page=32, dtype=dtype)
