@@ -16,9 +16,9 @@ int* gemm_status_word();   // device address of the status word shared with the 
 // ---------------------------------------------------------------------------------------------------------------------
 // attend_split_kernel: few query rows against many keys, kept to f32 accuracy.
 //
-// 64 sequences over 0.7k-8k keys (40 over 8 heads x 128, f16): 196 us a call = 6.1 TB/s (190 in a captured graph); on a bf16 cache
+// 64 sequences over 0.7k-8k keys (40 over 8 heads x 128, f16): 194 us a call = 6.1 TB/s (190 in a captured graph); on a bf16 cache
 // 229 in a graph: three parts of q and the sums pass the 168 registers that two CTAs per SM leave, and spill (288 bytes stored, 624
-// loaded).  One over 131000 (bf16): 116 us = 4.6 TB/s, of which the stream itself takes about 80.  Bound by the cache's bytes from
+// loaded).  One over 131000 (bf16): 114 us = 4.7 TB/s, of which the stream itself takes about 80.  Bound by the cache's bytes from
 // HBM (2 * 2 * head_dim per key and head; at 5 query heads per key-value head that is 5 multiply-adds per byte).  So: one CTA
 // reads a tile of 64 keys once for all query heads of its key-value head, tiles travel
 // by TMA into a ring filled by a warp of its own, and the line of all tiles is cut evenly over the resident CTAs

@@ -1,7 +1,7 @@
 // attend_prompt_kernel: attention of many new tokens (prompts and chunks of them), result in bf16, on tcgen05.
 //
-// A prompt of 4096 (40 over 8 heads x 128, bf16): 285 us a call = 603 TFLOP/s (267 in a captured graph); chunks of three prompts
-// (f16): 225 us = 841 TFLOP/s (208).  At head_dim 256 a prompt of 4096 (16 over 4 heads) takes 254 us in bf16, 202 in f16 (graph).
+// A prompt of 4096 (40 over 8 heads x 128, bf16): 288 us a call = 597 TFLOP/s (267 in a captured graph); chunks of three prompts
+// (f16): 227 us = 834 TFLOP/s (208).  At head_dim 256 a prompt of 4096 (16 over 4 heads) takes 254 us in bf16, 202 in f16 (graph).
 // Bound by the tensor cores (4 head_dim flop per visible pair and query head), short of it by a block's set-up and end and, in
 // bf16, by a ring of three stages.  A CTA takes 256 query rows (head_dim 256:
 // 128) of one key-value head -- (token, query head of the group) pairs, so that all heads of the group share the keys it
